@@ -320,6 +320,102 @@ qora_status qora_q4_lm_head(const float* d_x, const uint8_t* d_packed,
 
 
 /* ------------------------------------------------------------------------------------
+ * Many requests over one paged cache (no counterpart in the reference, whose RawKvCache
+ * holds one sequence): kernel-level entry points on DEVICE pointers for a host that keeps
+ * the K and V of many sequences in one pool of pages. They launch on `stream` of the
+ * current device, allocate nothing, do not synchronise, and may be captured into CUDA
+ * graphs; the arrays below are read when the kernels run, so a graph's next replay may find
+ * new contents in them.
+ *
+ * Rows. A row is one token: [heads][head_dim] contiguous elements, rows `stride` elements
+ * apart (stride >= heads * head_dim; pointers and strides on 16-byte boundaries), so that q,
+ * k and v may be parts of one joined row. head_dim is 64 or 128.
+ *
+ * Batch. Sequence s owns rows d_q_start[s] .. d_q_start[s+1] - 1 (seqs + 1 ascending
+ * numbers), its newest positions: with n of them and d_kv_len[s] = L positions in all (the
+ * new ones counted), its row i sits at position L - n + i. Sequences without new rows are
+ * allowed; rows that no sequence owns are left as they are.
+ *
+ * Pages. Position p of sequence s lies in page d_table[s * table_stride + p / page_size],
+ * slot p % page_size; element (page, head, slot, d) of the K (V) pages is at d_k_pages
+ * (d_v_pages) + page * page_stride + head * head_stride + slot * slot_stride + d (elements,
+ * multiples of 16 bytes). [page][slot][head][d] and [page][head][slot][d] are both taken,
+ * with any page_size. Table entries past a sequence's last position are not read.
+ *
+ * Types. Rows f32 with pages f32 or f16, rows and pages f16, rows and pages bf16. Sums,
+ * norms and softmax statistics are f32 throughout; a value is rounded once, to nearest
+ * even, where it is written (binary16 beyond +-65504 becomes infinite).
+ *
+ * What the host cannot see is checked on the device: a sequence whose rows lie outside
+ * [0, rows) or whose length does not fit its table row, a position behind the rotation
+ * tables, a page id outside [0, num_pages). What is out of range is skipped (its rows stay
+ * as they were; positions on a bad page count as masked) and *d_status (NULL: not
+ * reported) is set to QORA_ERR_RANGE. The library never clears *d_status.
+ * ---------------------------------------------------------------------------------- */
+#define QORA_DT_F32  0u
+#define QORA_DT_F16  1u
+#define QORA_DT_BF16 2u
+
+/* RMSNorm of each head of q and k and the split-half rotation in one pass (per head,
+ * rms_norm_f16 and apply_rope_raw, src/gemv.rs:744-778). Norms: q (k) heads are normalised
+ * when d_q_gamma (d_k_gamma), [head_dim] f32, is given. Rotation: d_cos and d_sin,
+ * [rope_rows][rope_half_dim] f32, both or neither; elements d and d + rope_half_dim turn
+ * together, elements from 2 * rope_half_dim on stay (rope_half_dim: a multiple of 8, at most
+ * head_dim / 2). d_pos: [rows]; a row with a negative position is padding and stays as it
+ * was. q_heads or kv_heads may be 0. Outputs may be the inputs themselves (equal strides). */
+qora_status qora_qk_norm_rope(const void* d_q, uint64_t q_stride, const void* d_k, uint64_t k_stride,
+                              uint32_t dtype, uint32_t rows, uint32_t q_heads, uint32_t kv_heads,
+                              uint32_t head_dim, const float* d_q_gamma, const float* d_k_gamma,
+                              float eps, const int32_t* d_pos, const float* d_cos,
+                              const float* d_sin, uint32_t rope_rows, uint32_t rope_half_dim,
+                              void* d_q_out, uint64_t q_out_stride, void* d_k_out,
+                              uint64_t k_out_stride, uint32_t* d_status, void* stream);
+
+/* Append the rows' k and v to the pages at their positions, k normalised and rotated on the
+ * way as in qora_qk_norm_rope (the position is the one the batch gives the row); q, when
+ * q_heads is not 0, goes through the same norm and rotation to d_q_out (which may be d_q).
+ * A row whose position is negative (L < n) has no place and is skipped, as out of range.
+ * No two rows may have the same place: two sequences may share pages, but not append to
+ * the same slot in one call (which of the rows such a slot then holds is not defined). */
+qora_status qora_paged_append(const void* d_q, uint64_t q_stride, const void* d_k, uint64_t k_stride,
+                              const void* d_v, uint64_t v_stride, uint32_t dtype, uint32_t rows,
+                              uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim,
+                              const float* d_q_gamma, const float* d_k_gamma, float eps,
+                              const float* d_cos, const float* d_sin, uint32_t rope_rows,
+                              uint32_t rope_half_dim, void* d_q_out, uint64_t q_out_stride,
+                              void* d_k_pages, void* d_v_pages, uint32_t kv_dtype,
+                              uint32_t num_pages, uint32_t page_size, uint64_t page_stride,
+                              uint64_t head_stride, uint64_t slot_stride,
+                              const int32_t* d_q_start, const int32_t* d_kv_len,
+                              const int32_t* d_table, uint32_t table_stride, uint32_t seqs,
+                              uint32_t* d_status, void* stream);
+
+/* Causal attention of every row over its sequence's pages (src/gemv.rs:914-989, for chunks
+ * of new rows and for single ones): row i of a sequence attends to positions
+ * max(0, p + 1 - window) .. p, p = L - n + i (window 0: from position 0), with weights
+ * softmax(scale * q . k); query head h reads kv head h / (q_heads / kv_heads). A row that
+ * attends to nothing gets zeros. What is masked does not count, whatever it holds (stale
+ * slots may hold infinities or NaN). d_lse (NULL: not written), [rows][q_heads] f32,
+ * receives log(sum exp(scale * q . k)), -inf for a row that attends to nothing. max_q: no
+ * sequence has more than max_q new rows (a longer one is out of range). scale > 0.
+ * d_work: QORA_PAGED_WORK_BYTES of scratch on a 256-byte boundary; its contents do not
+ * matter, and calls that may run at the same time (also replays of graphs that captured
+ * them) need a workspace each. Results are deterministic: the same call on the same
+ * contents gives the same bits. */
+#define QORA_PAGED_WORK_BYTES (64u * 1024u * 1024u)
+qora_status qora_paged_attention(const void* d_q, uint64_t q_stride, uint32_t dtype, uint32_t rows,
+                                 uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim,
+                                 float scale, uint32_t window, const void* d_k_pages,
+                                 const void* d_v_pages, uint32_t kv_dtype, uint32_t num_pages,
+                                 uint32_t page_size, uint64_t page_stride, uint64_t head_stride,
+                                 uint64_t slot_stride, const int32_t* d_q_start,
+                                 const int32_t* d_kv_len, const int32_t* d_table,
+                                 uint32_t table_stride, uint32_t seqs, uint32_t max_q, void* d_out,
+                                 uint64_t out_stride, float* d_lse, void* d_work,
+                                 uint64_t work_bytes, uint32_t* d_status, void* stream);
+
+
+/* ------------------------------------------------------------------------------------
  * Measurement entry points (no counterpart in the reference, which only times whole
  * calls with Instant, src/main.rs:105-117 and src/generate.rs:134-139, :255-260).
  * ---------------------------------------------------------------------------------- */

@@ -12,7 +12,7 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libqora_cuda.so")
-SOURCES = ["qora_engine.cu"]
+SOURCES = ["qora_engine.cu", "paged_ops.cu"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-O3", "-lineinfo", "-std=c++17",
@@ -20,6 +20,7 @@ NVCC_FLAGS = [
     "-Xptxas", "-O3",
     "--expt-relaxed-constexpr",
     "-cudart", "shared",
+    "--threads", "0",  # the translation units compile side by side
 ]
 
 

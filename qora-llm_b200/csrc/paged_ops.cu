@@ -1,0 +1,259 @@
+// paged_ops.cu — the kernel-level entry points for many requests over one paged cache:
+// qora_qk_norm_rope, qora_paged_append, qora_paged_attention (include/qora_cuda.h). All
+// checks that need no device data happen here; what lies in device memory (row ranges,
+// lengths, page ids) is checked by the kernels, which skip what is out of range and set
+// the caller's status word.
+#include <cmath>
+#include <cstdint>
+
+#include "host_util.h"
+#include "paged_attention.cuh"
+#include "paged_rows.cuh"
+
+using namespace qora;
+
+namespace {
+
+typedef unsigned long long ull;
+
+size_t elem_size(uint32_t dt) { return dt == QORA_DT_F32 ? 4 : 2; }
+
+qora_status check_types(uint32_t dtype, uint32_t kv_dtype) {
+  if (dtype > QORA_DT_BF16 || kv_dtype > QORA_DT_BF16)
+    return fail(QORA_ERR_INVALID, "element types %u and %u", dtype, kv_dtype);
+  if (dtype != kv_dtype && !(dtype == QORA_DT_F32 && kv_dtype == QORA_DT_F16))
+    return fail(QORA_ERR_UNSUPPORTED, "rows of type %u with a cache of type %u (equal types, or f32 rows with an f16 cache)",
+                dtype, kv_dtype);
+  return QORA_OK;
+}
+
+qora_status check_heads(uint32_t rows, uint32_t hq, uint32_t hk, uint32_t head_dim) {
+  if (head_dim != 64 && head_dim != 128) return fail(QORA_ERR_UNSUPPORTED, "head_dim %u: 64 or 128", head_dim);
+  if (hq > 1024 || hk > 1024) return fail(QORA_ERR_INVALID, "%u query heads, %u kv heads", hq, hk);
+  if (rows > (1u << 24)) return fail(QORA_ERR_INVALID, "%u rows in one call (at most 2^24)", rows);
+  return QORA_OK;
+}
+
+qora_status check_rows(const char* what, const void* p, uint64_t stride, uint32_t heads, uint32_t head_dim, size_t esz) {
+  if (!p) return fail(QORA_ERR_INVALID, "%s is NULL", what);
+  if (((uintptr_t)p | (stride * esz)) % 16)
+    return fail(QORA_ERR_INVALID, "%s: rows must start on 16-byte boundaries (stride %llu)", what, (ull)stride);
+  if (stride < (uint64_t)heads * head_dim || stride > (1ull << 40))
+    return fail(QORA_ERR_INVALID, "%s: row stride %llu for %u heads of %u", what, (ull)stride, heads, head_dim);
+  return QORA_OK;
+}
+
+qora_status check_same(const char* what, const void* in, uint64_t in_stride, const void* out, uint64_t out_stride) {
+  if (in == out && in_stride != out_stride)
+    return fail(QORA_ERR_INVALID, "%s in place needs equal strides (%llu, %llu)", what, (ull)in_stride, (ull)out_stride);
+  return QORA_OK;
+}
+
+qora_status check_turn(const float* q_gamma, const float* k_gamma, float eps, const float* cos_t, const float* sin_t,
+                       uint32_t rope_rows, uint32_t r, uint32_t head_dim) {
+  if (((uintptr_t)q_gamma | (uintptr_t)k_gamma | (uintptr_t)cos_t | (uintptr_t)sin_t) % 16)
+    return fail(QORA_ERR_INVALID, "gains and rotation tables must be 16-byte aligned");
+  if ((q_gamma || k_gamma) && !(eps >= 0.0f && std::isfinite(eps))) return fail(QORA_ERR_INVALID, "eps %g", (double)eps);
+  if (!cos_t != !sin_t) return fail(QORA_ERR_INVALID, "cos and sin tables go together");
+  if (cos_t) {
+    if (r == 0 || 2 * (uint64_t)r > head_dim) return fail(QORA_ERR_INVALID, "rope_half_dim %u for head_dim %u", r, head_dim);
+    if (r % 8) return fail(QORA_ERR_UNSUPPORTED, "rope_half_dim %u: a multiple of 8", r);
+    if (rope_rows == 0 || rope_rows > 0x7fffffffu) return fail(QORA_ERR_INVALID, "rope_rows %u", rope_rows);
+  }
+  return QORA_OK;
+}
+
+qora_status check_pages(const void* k, const void* v, uint32_t hk, uint32_t head_dim, size_t esz, uint32_t num_pages,
+                        uint32_t page_size, uint64_t page_stride, uint64_t head_stride, uint64_t slot_stride) {
+  if (!k || !v) return fail(QORA_ERR_INVALID, "NULL pages");
+  if (num_pages == 0 || num_pages > 0x7fffffffu || page_size == 0 || page_size > (1u << 20))
+    return fail(QORA_ERR_INVALID, "%u pages of %u positions", num_pages, page_size);
+  if (((uintptr_t)k | (uintptr_t)v | (page_stride * esz) | (head_stride * esz) | (slot_stride * esz)) % 16)
+    return fail(QORA_ERR_INVALID, "pages and their strides must be multiples of 16 bytes");
+  const uint64_t top = 1ull << 40;
+  if (page_stride > top || head_stride > top || slot_stride > top) return fail(QORA_ERR_INVALID, "page strides beyond 2^40");
+  const bool by_slot = slot_stride >= (uint64_t)(hk - 1) * head_stride + head_dim && (hk == 1 || head_stride >= head_dim);
+  const bool by_head = head_stride >= (uint64_t)(page_size - 1) * slot_stride + head_dim && (page_size == 1 || slot_stride >= head_dim);
+  if ((!by_slot && !by_head) ||
+      (num_pages > 1 && page_stride < (uint64_t)(page_size - 1) * slot_stride + (uint64_t)(hk - 1) * head_stride + head_dim))
+    return fail(QORA_ERR_INVALID, "page strides %llu, %llu, %llu overlap (page, head, slot)", (ull)page_stride,
+                (ull)head_stride, (ull)slot_stride);
+  return QORA_OK;
+}
+
+qora_status check_batch(const int32_t* q_start, const int32_t* kv_len, const int32_t* table, uint32_t table_stride,
+                        uint32_t page_size, uint32_t seqs) {
+  if (!q_start || !kv_len || !table) return fail(QORA_ERR_INVALID, "NULL batch arrays");
+  if (seqs > (1u << 20)) return fail(QORA_ERR_INVALID, "%u sequences", seqs);
+  if (table_stride == 0 || (uint64_t)table_stride * page_size > 0x7fffffffull)
+    return fail(QORA_ERR_INVALID, "table rows of %u pages of %u positions", table_stride, page_size);
+  return QORA_OK;
+}
+
+// Head rows a warp takes: one group where the launch is small (every load of the call in
+// flight at once), four where there are enough rows to fill the GPU either way.
+constexpr int kManyIters = 4;
+
+template <typename T, typename C, int D, bool kAppend>
+qora_status launch_rows(const paged::RowArgs& a, cudaStream_t s) {
+  constexpr int grp = 32 / (D / 2 / paged::Elem<T>::kVec);
+  const int heads = a.hq + a.hk + a.hv;
+  int dev = 0;
+  QCUDA(cudaGetDevice(&dev));
+  const long long one = (long long)a.rows * ((heads + grp - 1) / grp);
+  const bool many = one > 64LL * sm_count(dev);
+  const long long units = many ? (long long)a.rows * ((heads + grp * kManyIters - 1) / (grp * kManyIters)) : one;
+  const unsigned grid = (unsigned)((units + paged::kRowWarps - 1) / paged::kRowWarps);
+  if (many)
+    paged::rows_kernel<T, C, D, kManyIters, kAppend><<<grid, 32 * paged::kRowWarps, 0, s>>>(a);
+  else
+    paged::rows_kernel<T, C, D, 1, kAppend><<<grid, 32 * paged::kRowWarps, 0, s>>>(a);
+  QCUDA(cudaGetLastError());
+  return QORA_OK;
+}
+
+template <typename T, typename C, bool kAppend>
+qora_status launch_rows_d(uint32_t head_dim, const paged::RowArgs& a, cudaStream_t s) {
+  return head_dim == 64 ? launch_rows<T, C, 64, kAppend>(a, s) : launch_rows<T, C, 128, kAppend>(a, s);
+}
+
+template <typename T, typename C, int D>
+qora_status launch_attn(const paged::AttnArgs& a, cudaStream_t s) {
+  const long long units = (long long)a.batch.rows * a.hq;
+  paged::attn_row_kernel<T, C, D><<<(unsigned)((units + 7) / 8), 256, 0, s>>>(a);
+  QCUDA(cudaGetLastError());
+  return QORA_OK;
+}
+
+template <typename T, typename C>
+qora_status launch_attn_d(uint32_t head_dim, const paged::AttnArgs& a, cudaStream_t s) {
+  return head_dim == 64 ? launch_attn<T, C, 64>(a, s) : launch_attn<T, C, 128>(a, s);
+}
+
+}  // namespace
+
+extern "C" {
+
+qora_status qora_qk_norm_rope(const void* d_q, uint64_t q_stride, const void* d_k, uint64_t k_stride, uint32_t dtype,
+                              uint32_t rows, uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim,
+                              const float* d_q_gamma, const float* d_k_gamma, float eps, const int32_t* d_pos,
+                              const float* d_cos, const float* d_sin, uint32_t rope_rows, uint32_t rope_half_dim,
+                              void* d_q_out, uint64_t q_out_stride, void* d_k_out, uint64_t k_out_stride,
+                              uint32_t* d_status, void* stream) {
+  QCHECK(check_types(dtype, dtype));
+  QCHECK(check_heads(rows, q_heads, kv_heads, head_dim));
+  if (q_heads + kv_heads == 0) return fail(QORA_ERR_INVALID, "no heads");
+  const size_t esz = elem_size(dtype);
+  if (q_heads) {
+    QCHECK(check_rows("q", d_q, q_stride, q_heads, head_dim, esz));
+    QCHECK(check_rows("q_out", d_q_out, q_out_stride, q_heads, head_dim, esz));
+    QCHECK(check_same("q", d_q, q_stride, d_q_out, q_out_stride));
+  }
+  if (kv_heads) {
+    QCHECK(check_rows("k", d_k, k_stride, kv_heads, head_dim, esz));
+    QCHECK(check_rows("k_out", d_k_out, k_out_stride, kv_heads, head_dim, esz));
+    QCHECK(check_same("k", d_k, k_stride, d_k_out, k_out_stride));
+  }
+  QCHECK(check_turn(d_q_gamma, d_k_gamma, eps, d_cos, d_sin, rope_rows, rope_half_dim, head_dim));
+  if (d_cos && !d_pos) return fail(QORA_ERR_INVALID, "a rotation needs positions");
+  if (rows == 0) return QORA_OK;
+  paged::RowArgs a{};
+  a.q = d_q, a.k = d_k, a.q_stride = (long long)q_stride, a.k_stride = (long long)k_stride;
+  a.rows = (int)rows, a.hq = (int)q_heads, a.hk = (int)kv_heads, a.hv = 0;
+  a.q_gamma = d_q_gamma, a.k_gamma = d_k_gamma, a.eps = eps;
+  a.pos = d_pos, a.cos_t = d_cos, a.sin_t = d_sin, a.rope_rows = (int)rope_rows;
+  a.r = d_cos ? (int)rope_half_dim : (int)head_dim / 2;
+  a.q_out = d_q_out, a.k_out = d_k_out, a.qo_stride = (long long)q_out_stride, a.ko_stride = (long long)k_out_stride;
+  a.status = d_status;
+  const cudaStream_t s = (cudaStream_t)stream;
+  if (dtype == QORA_DT_F32) return launch_rows_d<float, float, false>(head_dim, a, s);
+  if (dtype == QORA_DT_F16) return launch_rows_d<__half, __half, false>(head_dim, a, s);
+  return launch_rows_d<__nv_bfloat16, __nv_bfloat16, false>(head_dim, a, s);
+}
+
+qora_status qora_paged_append(const void* d_q, uint64_t q_stride, const void* d_k, uint64_t k_stride, const void* d_v,
+                              uint64_t v_stride, uint32_t dtype, uint32_t rows, uint32_t q_heads, uint32_t kv_heads,
+                              uint32_t head_dim, const float* d_q_gamma, const float* d_k_gamma, float eps,
+                              const float* d_cos, const float* d_sin, uint32_t rope_rows, uint32_t rope_half_dim,
+                              void* d_q_out, uint64_t q_out_stride, void* d_k_pages, void* d_v_pages, uint32_t kv_dtype,
+                              uint32_t num_pages, uint32_t page_size, uint64_t page_stride, uint64_t head_stride,
+                              uint64_t slot_stride, const int32_t* d_q_start, const int32_t* d_kv_len,
+                              const int32_t* d_table, uint32_t table_stride, uint32_t seqs, uint32_t* d_status,
+                              void* stream) {
+  QCHECK(check_types(dtype, kv_dtype));
+  QCHECK(check_heads(rows, q_heads, kv_heads, head_dim));
+  if (kv_heads == 0) return fail(QORA_ERR_INVALID, "no kv heads");
+  const size_t esz = elem_size(dtype);
+  if (q_heads) {
+    QCHECK(check_rows("q", d_q, q_stride, q_heads, head_dim, esz));
+    QCHECK(check_rows("q_out", d_q_out, q_out_stride, q_heads, head_dim, esz));
+    QCHECK(check_same("q", d_q, q_stride, d_q_out, q_out_stride));
+  }
+  QCHECK(check_rows("k", d_k, k_stride, kv_heads, head_dim, esz));
+  QCHECK(check_rows("v", d_v, v_stride, kv_heads, head_dim, esz));
+  QCHECK(check_turn(d_q_gamma, d_k_gamma, eps, d_cos, d_sin, rope_rows, rope_half_dim, head_dim));
+  QCHECK(check_pages(d_k_pages, d_v_pages, kv_heads, head_dim, elem_size(kv_dtype), num_pages, page_size, page_stride,
+                     head_stride, slot_stride));
+  QCHECK(check_batch(d_q_start, d_kv_len, d_table, table_stride, page_size, seqs));
+  if (rows == 0 || seqs == 0) return QORA_OK;
+  paged::RowArgs a{};
+  a.q = d_q, a.k = d_k, a.v = d_v;
+  a.q_stride = (long long)q_stride, a.k_stride = (long long)k_stride, a.v_stride = (long long)v_stride;
+  a.rows = (int)rows, a.hq = (int)q_heads, a.hk = a.hv = (int)kv_heads;
+  a.q_gamma = q_heads ? d_q_gamma : nullptr, a.k_gamma = d_k_gamma, a.eps = eps;
+  a.cos_t = d_cos, a.sin_t = d_sin, a.rope_rows = (int)rope_rows;
+  a.r = d_cos ? (int)rope_half_dim : (int)head_dim / 2;
+  a.q_out = d_q_out, a.qo_stride = (long long)q_out_stride;
+  a.k_pages = d_k_pages, a.v_pages = d_v_pages;
+  a.pg = {(int)num_pages, (int)page_size, (long long)page_stride, (long long)head_stride, (long long)slot_stride};
+  a.batch = {d_q_start, d_kv_len, d_table, (int)table_stride, (int)seqs, (int)rows};
+  a.status = d_status;
+  const cudaStream_t s = (cudaStream_t)stream;
+  if (dtype == QORA_DT_F32 && kv_dtype == QORA_DT_F32) return launch_rows_d<float, float, true>(head_dim, a, s);
+  if (dtype == QORA_DT_F32) return launch_rows_d<float, __half, true>(head_dim, a, s);
+  if (dtype == QORA_DT_F16) return launch_rows_d<__half, __half, true>(head_dim, a, s);
+  return launch_rows_d<__nv_bfloat16, __nv_bfloat16, true>(head_dim, a, s);
+}
+
+qora_status qora_paged_attention(const void* d_q, uint64_t q_stride, uint32_t dtype, uint32_t rows, uint32_t q_heads,
+                                 uint32_t kv_heads, uint32_t head_dim, float scale, uint32_t window,
+                                 const void* d_k_pages, const void* d_v_pages, uint32_t kv_dtype, uint32_t num_pages,
+                                 uint32_t page_size, uint64_t page_stride, uint64_t head_stride, uint64_t slot_stride,
+                                 const int32_t* d_q_start, const int32_t* d_kv_len, const int32_t* d_table,
+                                 uint32_t table_stride, uint32_t seqs, uint32_t max_q, void* d_out, uint64_t out_stride,
+                                 float* d_lse, void* d_work, uint64_t work_bytes, uint32_t* d_status, void* stream) {
+  QCHECK(check_types(dtype, kv_dtype));
+  QCHECK(check_heads(rows, q_heads, kv_heads, head_dim));
+  if (kv_heads == 0 || q_heads == 0 || q_heads % kv_heads || q_heads / kv_heads > 128)
+    return fail(QORA_ERR_INVALID, "%u query heads over %u kv heads", q_heads, kv_heads);
+  const size_t esz = elem_size(dtype);
+  QCHECK(check_rows("q", d_q, q_stride, q_heads, head_dim, esz));
+  QCHECK(check_rows("out", d_out, out_stride, q_heads, head_dim, esz));
+  if (!(scale > 0.0f) || !std::isfinite(scale)) return fail(QORA_ERR_INVALID, "scale %g", (double)scale);
+  if (window > 0x7fffffffu) return fail(QORA_ERR_INVALID, "window %u", window);
+  QCHECK(check_pages(d_k_pages, d_v_pages, kv_heads, head_dim, elem_size(kv_dtype), num_pages, page_size, page_stride,
+                     head_stride, slot_stride));
+  QCHECK(check_batch(d_q_start, d_kv_len, d_table, table_stride, page_size, seqs));
+  if (!d_work || (uintptr_t)d_work % 256 || work_bytes < QORA_PAGED_WORK_BYTES)
+    return fail(QORA_ERR_INVALID, "the workspace needs %u bytes on a 256-byte boundary", QORA_PAGED_WORK_BYTES);
+  if (rows == 0 || seqs == 0) return QORA_OK;
+  if (max_q == 0) return fail(QORA_ERR_INVALID, "max_q is 0");
+  paged::AttnArgs a{};
+  a.q = d_q, a.q_stride = (long long)q_stride;
+  a.out = d_out, a.out_stride = (long long)out_stride;
+  a.lse = d_lse;
+  a.k_pages = d_k_pages, a.v_pages = d_v_pages;
+  a.pg = {(int)num_pages, (int)page_size, (long long)page_stride, (long long)head_stride, (long long)slot_stride};
+  a.batch = {d_q_start, d_kv_len, d_table, (int)table_stride, (int)seqs, (int)rows};
+  a.hq = (int)q_heads, a.hk = (int)kv_heads, a.group = (int)(q_heads / kv_heads);
+  a.window = (int)window, a.scale = scale;
+  a.max_q = (int)(max_q < rows ? max_q : rows);
+  a.status = d_status;
+  const cudaStream_t s = (cudaStream_t)stream;
+  if (dtype == QORA_DT_F32 && kv_dtype == QORA_DT_F32) return launch_attn_d<float, float>(head_dim, a, s);
+  if (dtype == QORA_DT_F32) return launch_attn_d<float, __half>(head_dim, a, s);
+  if (dtype == QORA_DT_F16) return launch_attn_d<__half, __half>(head_dim, a, s);
+  return launch_attn_d<__nv_bfloat16, __nv_bfloat16>(head_dim, a, s);
+}
+
+}  // extern "C"

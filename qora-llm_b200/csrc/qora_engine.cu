@@ -14,7 +14,6 @@
 #include <algorithm>
 #include <atomic>
 #include <cmath>
-#include <cstdarg>
 #include <cstdio>
 #include <fcntl.h>
 #include <sys/mman.h>
@@ -34,6 +33,7 @@
 #include "attention.cuh"
 #include "common.cuh"
 #include "f16_batch.cuh"
+#include "host_util.h"
 #include "lm_head.cuh"
 #include "umma_gemm.cuh"
 #include "megakernel.cuh"
@@ -45,38 +45,6 @@
 using namespace qora;
 
 namespace {
-
-thread_local std::string g_last_error;
-
-qora_status fail(qora_status st, const char* fmt, ...) {
-  char buf[1024];
-  va_list ap;
-  va_start(ap, fmt);
-  std::vsnprintf(buf, sizeof(buf), fmt, ap);
-  va_end(ap);
-  g_last_error = buf;
-  return st;
-}
-
-#define QCUDA(call)                                                                   \
-  do {                                                                                \
-    cudaError_t e_ = (call);                                                          \
-    if (e_ != cudaSuccess)                                                            \
-      return fail(e_ == cudaErrorMemoryAllocation ? QORA_ERR_OOM : QORA_ERR_CUDA,     \
-                  "%s failed: %s (%s:%d)", #call, cudaGetErrorString(e_), __FILE__, __LINE__); \
-  } while (0)
-
-#define QCHECK(expr)                 \
-  do {                               \
-    qora_status s_ = (expr);         \
-    if (s_ != QORA_OK) return s_;    \
-  } while (0)
-
-int sm_count(int dev) {
-  int n = 0;
-  cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
-  return n > 0 ? n : 148;
-}
 
 // ------------------------------------------------------------------ GEMV planning
 struct GemvShape {

@@ -70,6 +70,17 @@ SIGNATURES = {
     "qora_q4_gate_up": (C.c_int, [_vp, _vp, _vp, _vp, _vp, _u64, _u64, _vp, _vp]),
     "qora_q4_lm_head": (C.c_int, [_vp, _vp, _vp, _u64, _u64, _vp, _vp, _vp]),
     "qora_f16_gemm": (C.c_int, [_vp, _vp, _u64, _u64, _u64, _vp, _vp]),
+    "qora_qk_norm_rope": (C.c_int, [_vp, _u64, _vp, _u64, _u32, _u32, _u32, _u32, _u32, _vp, _vp,
+                                    C.c_float, _vp, _vp, _vp, _u32, _u32, _vp, _u64, _vp, _u64,
+                                    _vp, _vp]),
+    "qora_paged_append": (C.c_int, [_vp, _u64, _vp, _u64, _vp, _u64, _u32, _u32, _u32, _u32, _u32,
+                                    _vp, _vp, C.c_float, _vp, _vp, _u32, _u32, _vp, _u64, _vp,
+                                    _vp, _u32, _u32, _u32, _u64, _u64, _u64, _vp, _vp, _vp, _u32,
+                                    _u32, _vp, _vp]),
+    "qora_paged_attention": (C.c_int, [_vp, _u64, _u32, _u32, _u32, _u32, _u32, C.c_float, _u32,
+                                       _vp, _vp, _u32, _u32, _u32, _u64, _u64, _u64, _vp, _vp,
+                                       _vp, _u32, _u32, _u32, _vp, _u64, _vp, _vp, _u64, _vp,
+                                       _vp]),
     "qora_sample": (C.c_int, [_vp, _u32, _vp, _u32, _vp, _P(_u64), _P(_u32)]),
     "qora_sample_logits": (C.c_int, [_vp, _u32, _vp, _u32, _vp, _P(_u64), _P(_u32), _vp]),
 }
@@ -388,6 +399,63 @@ def sample_logits(logits_ptr, vocab, history_ptr, n_history, temperature, top_p,
     check(lib().qora_sample_logits(logits_ptr, vocab, history_ptr, n_history, C.byref(p), C.byref(st),
                                    C.byref(tok), _stream_ptr(stream)))
     return tok.value, st.value
+
+
+DTYPES = {"f32": 0, "f16": 1, "bf16": 2}  # QORA_DT_*
+PAGED_WORK_BYTES = 64 << 20  # QORA_PAGED_WORK_BYTES
+
+
+def _dtype(name):
+    try:
+        return DTYPES[name]
+    except KeyError:
+        raise ValueError(f"element type {name!r}: one of {sorted(DTYPES)}") from None
+
+
+def qk_norm_rope(q_ptr, k_ptr, q_out_ptr, k_out_ptr, rows, q_heads, kv_heads, head_dim, pos_ptr, cos_ptr, sin_ptr,
+                 rope_rows, rope_half_dim, q_gamma_ptr=None, k_gamma_ptr=None, eps=1e-6, dtype="f32", q_stride=None,
+                 k_stride=None, q_out_stride=None, k_out_stride=None, status_ptr=None, stream=None):
+    """RMSNorm of each head of q and k (with gains) and the rotation, in one pass
+    (qora_qk_norm_rope). Strides are elements from one row to the next (default: no gap)."""
+    nq, nk = q_heads * head_dim, kv_heads * head_dim
+    check(lib().qora_qk_norm_rope(
+        q_ptr, nq if q_stride is None else q_stride, k_ptr, nk if k_stride is None else k_stride, _dtype(dtype), rows,
+        q_heads, kv_heads, head_dim, q_gamma_ptr, k_gamma_ptr, eps, pos_ptr, cos_ptr, sin_ptr, rope_rows,
+        rope_half_dim, q_out_ptr, nq if q_out_stride is None else q_out_stride, k_out_ptr,
+        nk if k_out_stride is None else k_out_stride, status_ptr, _stream_ptr(stream)))
+
+
+def paged_append(k_ptr, v_ptr, rows, kv_heads, head_dim, k_pages_ptr, v_pages_ptr, num_pages, page_size, q_start_ptr,
+                 kv_len_ptr, table_ptr, table_stride, seqs, q_ptr=None, q_out_ptr=None, q_heads=0, cos_ptr=None,
+                 sin_ptr=None, rope_rows=0, rope_half_dim=0, q_gamma_ptr=None, k_gamma_ptr=None, eps=1e-6, dtype="f32",
+                 kv_dtype="f32", q_stride=None, k_stride=None, v_stride=None, q_out_stride=None, page_strides=None,
+                 status_ptr=None, stream=None):
+    """Append k and v rows to a paged cache, k (and q, to q_out) normalised and rotated on
+    the way (qora_paged_append). page_strides: elements per (page, head, slot); default
+    [page][head][slot][head_dim], the head-major order of KVCache."""
+    nq, nk = q_heads * head_dim, kv_heads * head_dim
+    ps, hs, ss = page_strides or (page_size * nk, page_size * head_dim, head_dim)
+    check(lib().qora_paged_append(
+        q_ptr, nq if q_stride is None else q_stride, k_ptr, nk if k_stride is None else k_stride, v_ptr,
+        nk if v_stride is None else v_stride, _dtype(dtype), rows, q_heads, kv_heads, head_dim, q_gamma_ptr,
+        k_gamma_ptr, eps, cos_ptr, sin_ptr, rope_rows, rope_half_dim, q_out_ptr,
+        nq if q_out_stride is None else q_out_stride, k_pages_ptr, v_pages_ptr, _dtype(kv_dtype), num_pages, page_size,
+        ps, hs, ss, q_start_ptr, kv_len_ptr, table_ptr, table_stride, seqs, status_ptr, _stream_ptr(stream)))
+
+
+def paged_attention(q_ptr, out_ptr, rows, q_heads, kv_heads, head_dim, k_pages_ptr, v_pages_ptr, num_pages, page_size,
+                    q_start_ptr, kv_len_ptr, table_ptr, table_stride, seqs, max_q, work_ptr,
+                    work_bytes=PAGED_WORK_BYTES, scale=None, window=0, lse_ptr=None, dtype="f32", kv_dtype="f32",
+                    q_stride=None, out_stride=None, page_strides=None, status_ptr=None, stream=None):
+    """Causal attention of each sequence's newest rows over its pages (qora_paged_attention).
+    scale: default 1 / sqrt(head_dim); page_strides as in paged_append."""
+    nq, nk = q_heads * head_dim, kv_heads * head_dim
+    ps, hs, ss = page_strides or (page_size * nk, page_size * head_dim, head_dim)
+    check(lib().qora_paged_attention(
+        q_ptr, nq if q_stride is None else q_stride, _dtype(dtype), rows, q_heads, kv_heads, head_dim,
+        max(head_dim, 1) ** -0.5 if scale is None else scale, window, k_pages_ptr, v_pages_ptr, _dtype(kv_dtype), num_pages,
+        page_size, ps, hs, ss, q_start_ptr, kv_len_ptr, table_ptr, table_stride, seqs, max_q, out_ptr,
+        nq if out_stride is None else out_stride, lse_ptr, work_ptr, work_bytes, status_ptr, _stream_ptr(stream)))
 
 
 def tp_plan(fmt: int, num_heads: int, num_kv_heads: int, intermediate: int, vocab: int, tp: int, rank: int) -> dict:

@@ -31,6 +31,10 @@ pub const QORA_KV_F32: u32 = 0;
 pub const QORA_KV_F16: u32 = 1;
 pub const QORA_GEMV_STATIC_FLOATS: u32 = 512 * 1024;
 pub const QORA_GEMV_STATIC_TILES: u32 = 1024;
+pub const QORA_DT_F32: u32 = 0;
+pub const QORA_DT_F16: u32 = 1;
+pub const QORA_DT_BF16: u32 = 2;
+pub const QORA_PAGED_WORK_BYTES: u32 = 64 * 1024 * 1024;
 
 pub const QORA_KERNEL_QKV: c_int = 0;
 pub const QORA_KERNEL_ATTENTION: c_int = 1;
@@ -301,6 +305,100 @@ extern "C" {
         hidden: u64,
         d_logits: *mut f32,
         d_argmax: *mut u32,
+        stream: *mut c_void,
+    ) -> qora_status;
+    pub fn qora_qk_norm_rope(
+        d_q: *const c_void,
+        q_stride: u64,
+        d_k: *const c_void,
+        k_stride: u64,
+        dtype: u32,
+        rows: u32,
+        q_heads: u32,
+        kv_heads: u32,
+        head_dim: u32,
+        d_q_gamma: *const f32,
+        d_k_gamma: *const f32,
+        eps: f32,
+        d_pos: *const i32,
+        d_cos: *const f32,
+        d_sin: *const f32,
+        rope_rows: u32,
+        rope_half_dim: u32,
+        d_q_out: *mut c_void,
+        q_out_stride: u64,
+        d_k_out: *mut c_void,
+        k_out_stride: u64,
+        d_status: *mut u32,
+        stream: *mut c_void,
+    ) -> qora_status;
+    pub fn qora_paged_append(
+        d_q: *const c_void,
+        q_stride: u64,
+        d_k: *const c_void,
+        k_stride: u64,
+        d_v: *const c_void,
+        v_stride: u64,
+        dtype: u32,
+        rows: u32,
+        q_heads: u32,
+        kv_heads: u32,
+        head_dim: u32,
+        d_q_gamma: *const f32,
+        d_k_gamma: *const f32,
+        eps: f32,
+        d_cos: *const f32,
+        d_sin: *const f32,
+        rope_rows: u32,
+        rope_half_dim: u32,
+        d_q_out: *mut c_void,
+        q_out_stride: u64,
+        d_k_pages: *mut c_void,
+        d_v_pages: *mut c_void,
+        kv_dtype: u32,
+        num_pages: u32,
+        page_size: u32,
+        page_stride: u64,
+        head_stride: u64,
+        slot_stride: u64,
+        d_q_start: *const i32,
+        d_kv_len: *const i32,
+        d_table: *const i32,
+        table_stride: u32,
+        seqs: u32,
+        d_status: *mut u32,
+        stream: *mut c_void,
+    ) -> qora_status;
+    pub fn qora_paged_attention(
+        d_q: *const c_void,
+        q_stride: u64,
+        dtype: u32,
+        rows: u32,
+        q_heads: u32,
+        kv_heads: u32,
+        head_dim: u32,
+        scale: f32,
+        window: u32,
+        d_k_pages: *const c_void,
+        d_v_pages: *const c_void,
+        kv_dtype: u32,
+        num_pages: u32,
+        page_size: u32,
+        page_stride: u64,
+        head_stride: u64,
+        slot_stride: u64,
+        d_q_start: *const i32,
+        d_kv_len: *const i32,
+        d_table: *const i32,
+        table_stride: u32,
+        seqs: u32,
+        max_q: u32,
+        d_out: *mut c_void,
+        out_stride: u64,
+        d_lse: *mut f32,
+        d_work: *mut c_void,
+        work_bytes: u64,
+        d_status: *mut u32,
         stream: *mut c_void,
     ) -> qora_status;
     pub fn qora_generate_greedy_timed(
