@@ -3,12 +3,15 @@
 // checks that need no device data happen here; what lies in device memory (row ranges,
 // lengths, page ids) is checked by the kernels, which skip what is out of range and set
 // the caller's status word.
+#include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <cstdint>
 
 #include "host_util.h"
 #include "paged_attention.cuh"
 #include "paged_rows.cuh"
+#include "paged_token.cuh"
 
 using namespace qora;
 
@@ -117,8 +120,45 @@ qora_status launch_rows_d(uint32_t head_dim, const paged::RowArgs& a, cudaStream
   return head_dim == 64 ? launch_rows<T, C, 64, kAppend>(a, s) : launch_rows<T, C, 128, kAppend>(a, s);
 }
 
+// A kernel's dynamic shared memory limit, set once per device and kernel.
+template <auto* kKernel>
+qora_status allow_smem(int dev, int bytes) {
+  static std::atomic<uint64_t> done{0};
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (done.load(std::memory_order_acquire) & bit) return QORA_OK;
+  QCUDA(cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  done.fetch_or(bit, std::memory_order_release);
+  return QORA_OK;
+}
+
+// Fewest steps worth a CTA of their own: one per warp.
+constexpr int kTokenMinSteps = 8;
+
 template <typename T, typename C, int D>
-qora_status launch_attn(const paged::AttnArgs& a, cudaStream_t s) {
+qora_status launch_token(const paged::AttnArgs& a, void* work, cudaStream_t s) {
+  using Cfg = paged::TokenCfg<T, C, D>;
+  int dev = 0;
+  QCUDA(cudaGetDevice(&dev));
+  QCHECK((allow_smem<&paged::token_kernel<T, C, D>>(dev, Cfg::kSmem)));
+  const int ctas = std::min(sm_count(dev), paged::kTokenMaxCtas);
+  paged::token_kernel<T, C, D><<<ctas, 32 * Cfg::kWarps, Cfg::kSmem, s>>>(a, work, kTokenMinSteps);
+  QCUDA(cudaGetLastError());
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ctas, std::min<long long>(Cfg::kRows, (long long)a.max_q * a.group));
+  cfg.blockDim = dim3(128);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  QCUDA(cudaLaunchKernelEx(&cfg, paged::token_join_kernel<T, D, Cfg::kRows>, a, work, ctas));
+  return QORA_OK;
+}
+
+template <typename T, typename C, int D>
+qora_status launch_attn(const paged::AttnArgs& a, void* work, cudaStream_t s) {
+  if ((long long)a.max_q * a.group <= paged::TokenCfg<T, C, D>::kRows) return launch_token<T, C, D>(a, work, s);
   const long long units = (long long)a.batch.rows * a.hq;
   paged::attn_row_kernel<T, C, D><<<(unsigned)((units + 7) / 8), 256, 0, s>>>(a);
   QCUDA(cudaGetLastError());
@@ -126,8 +166,8 @@ qora_status launch_attn(const paged::AttnArgs& a, cudaStream_t s) {
 }
 
 template <typename T, typename C>
-qora_status launch_attn_d(uint32_t head_dim, const paged::AttnArgs& a, cudaStream_t s) {
-  return head_dim == 64 ? launch_attn<T, C, 64>(a, s) : launch_attn<T, C, 128>(a, s);
+qora_status launch_attn_d(uint32_t head_dim, const paged::AttnArgs& a, void* work, cudaStream_t s) {
+  return head_dim == 64 ? launch_attn<T, C, 64>(a, work, s) : launch_attn<T, C, 128>(a, work, s);
 }
 
 }  // namespace
@@ -250,10 +290,10 @@ qora_status qora_paged_attention(const void* d_q, uint64_t q_stride, uint32_t dt
   a.max_q = (int)(max_q < rows ? max_q : rows);
   a.status = d_status;
   const cudaStream_t s = (cudaStream_t)stream;
-  if (dtype == QORA_DT_F32 && kv_dtype == QORA_DT_F32) return launch_attn_d<float, float>(head_dim, a, s);
-  if (dtype == QORA_DT_F32) return launch_attn_d<float, __half>(head_dim, a, s);
-  if (dtype == QORA_DT_F16) return launch_attn_d<__half, __half>(head_dim, a, s);
-  return launch_attn_d<__nv_bfloat16, __nv_bfloat16>(head_dim, a, s);
+  if (dtype == QORA_DT_F32 && kv_dtype == QORA_DT_F32) return launch_attn_d<float, float>(head_dim, a, d_work, s);
+  if (dtype == QORA_DT_F32) return launch_attn_d<float, __half>(head_dim, a, d_work, s);
+  if (dtype == QORA_DT_F16) return launch_attn_d<__half, __half>(head_dim, a, d_work, s);
+  return launch_attn_d<__nv_bfloat16, __nv_bfloat16>(head_dim, a, d_work, s);
 }
 
 }  // extern "C"
