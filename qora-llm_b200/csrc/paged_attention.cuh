@@ -21,6 +21,7 @@ struct AttnArgs {
   Pages pg;
   Batch batch;
   int hq, hk, group;  // group = hq / hk
+  int group_inv;      // ceil(2^16 / group)
   int window;         // 0: none
   int max_q;          // no sequence has more new rows
   float scale;

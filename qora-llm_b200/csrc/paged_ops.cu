@@ -131,8 +131,9 @@ qora_status allow_smem(int dev, int bytes) {
   return QORA_OK;
 }
 
-// Fewest steps worth a CTA of their own: one per warp.
-constexpr int kTokenMinSteps = 8;
+// Fewest units of work worth a CTA of their own, and what a tile's fixed time counts, in steps.
+constexpr int kTokenMinSteps = 16;
+constexpr int kTokenTileCost = 16;
 
 template <typename T, typename C, int D>
 qora_status launch_token(const paged::AttnArgs& a, void* work, cudaStream_t s) {
@@ -140,8 +141,9 @@ qora_status launch_token(const paged::AttnArgs& a, void* work, cudaStream_t s) {
   int dev = 0;
   QCUDA(cudaGetDevice(&dev));
   QCHECK((allow_smem<&paged::token_kernel<T, C, D>>(dev, Cfg::kSmem)));
+  QCHECK((allow_smem<&paged::token_join_kernel<T, D>>(dev, 0)));
   const int ctas = std::min(sm_count(dev), paged::kTokenMaxCtas);
-  paged::token_kernel<T, C, D><<<ctas, 32 * Cfg::kWarps, Cfg::kSmem, s>>>(a, work, kTokenMinSteps);
+  paged::token_kernel<T, C, D><<<ctas, 32 * Cfg::kWarps, Cfg::kSmem, s>>>(a, work, kTokenMinSteps, kTokenTileCost);
   QCUDA(cudaGetLastError());
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(ctas, std::min<long long>(Cfg::kRows, (long long)a.max_q * a.group));
@@ -152,7 +154,7 @@ qora_status launch_token(const paged::AttnArgs& a, void* work, cudaStream_t s) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  QCUDA(cudaLaunchKernelEx(&cfg, paged::token_join_kernel<T, D, Cfg::kRows>, a, work, ctas));
+  QCUDA(cudaLaunchKernelEx(&cfg, paged::token_join_kernel<T, D>, a, work, ctas));
   return QORA_OK;
 }
 
@@ -286,6 +288,7 @@ qora_status qora_paged_attention(const void* d_q, uint64_t q_stride, uint32_t dt
   a.pg = {(int)num_pages, (int)page_size, (long long)page_stride, (long long)head_stride, (long long)slot_stride};
   a.batch = {d_q_start, d_kv_len, d_table, (int)table_stride, (int)seqs, (int)rows};
   a.hq = (int)q_heads, a.hk = (int)kv_heads, a.group = (int)(q_heads / kv_heads);
+  a.group_inv = (65535 + a.group) / a.group;
   a.window = (int)window, a.scale = scale;
   a.max_q = (int)(max_q < rows ? max_q : rows);
   a.status = d_status;

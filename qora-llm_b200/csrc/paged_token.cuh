@@ -3,8 +3,7 @@
 //
 // Tile. A tile is one (sequence, kv head): its rows are the sequence's new tokens times the
 // kv head's query heads, packed (row r: token r / group, head r % group), at most kRows of
-// them (longer ones: several tiles that share the positions through L2). kRows is what one
-// m16 matrix instruction holds: 16 rows of 16-bit q, or 8 rows of f32 q, whose binary16
+// them. kRows is what one m16 matrix instruction holds: 16 rows of 16-bit q, or 8 rows of f32 q, whose binary16
 // (tf32, for an f32 cache) upper and lower halves are the instruction's rows 0-7 and 8-15:
 // the 22 bits cost no second instruction. An f32 cache is split likewise into two operands.
 //
@@ -28,6 +27,7 @@
 #pragma once
 
 #include "paged_attention.cuh"
+#include "ptx.cuh"
 
 namespace qora {
 namespace paged {
@@ -84,6 +84,9 @@ QORA_DEV void mma_tf32(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint3
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// token of packed row r (< 16) of a tile: r / group
+QORA_DEV int token_of(const AttnArgs& a, int r) { return (r * a.group_inv) >> 16; }
+
 QORA_DEV uint32_t pack2(float a, float b, __half) {
   const __half2 h = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&h);
@@ -103,13 +106,21 @@ struct TokenCfg {
   static constexpr bool kHalves = sizeof(T) == 4;   // f32 rows: upper and lower halves
   static constexpr int kRows = kHalves ? 8 : 16;
   static constexpr int kPos = kWide ? 8 : 16;       // positions of a step
-  static constexpr int kChunks = D * (int)sizeof(C) / 16;  // 16-byte pieces of a K or V row
-  static constexpr int kSide = kPos * kChunks * 16;        // bytes of a step's K (or V)
+  static constexpr int kRowBytes = D * (int)sizeof(C);
+  static constexpr int kChunks = kRowBytes / 16;    // 16-byte pieces of a K or V row
+  // Pieces are permuted within their 128 bytes so that the reads below touch every bank once:
+  // ldmatrix reads one piece of 8 rows; a quarter-warp reads 4 pieces of 2 rows of an f32 K
+  // and 2 pieces of rows 0, 2, 4, 6 of V. (Rows padded by 16 bytes instead: 225 us where
+  // this takes 196 us, 128 tokens over 4,100 positions each; the copies write whole lines.)
+  QORA_DEV static int k_at(int row, int ch) { return row * kRowBytes + ((kWide ? ch ^ ((row & 1) << 2) : ch ^ (row & 7)) << 4); }
+  QORA_DEV static int v_at(int row, int ch) { return row * kRowBytes + ((kWide ? ch ^ (row & 6) : ch ^ (row & 7)) << 4); }
+  static constexpr int kSide = kPos * kRowBytes;  // bytes of a step's K (or V)
+  static constexpr int kStep = 2 * kSide;
   static constexpr int kStages = 3;
   static constexpr int kWarps = 8;
-  static constexpr int kRing = kStages * 2 * kSide;  // bytes of a warp's ring
-  static constexpr int kStage_ = kRows * D * 4;      // a warp's numerators at a segment's end, in its ring
-  static_assert(kStage_ <= kRing, "the ring holds the numerators");
+  static constexpr int kRing = kStages * kStep;  // bytes of a warp's ring
+  static constexpr int kNum = D + (kWide ? 4 : 8);  // floats from one row of numerators to the next, in the ring
+  static_assert(kRows * kNum * 4 <= kRing, "the ring holds the numerators");
   static constexpr int kSmem = kWarps * kRing;
 };
 
@@ -118,7 +129,7 @@ constexpr int kTokenMaxRows = 16;
 
 // Workspace: records [ctas], partial maxima and sums [2 ctas][16], numerators [2 ctas][16][D].
 struct TokenWork {
-  int4* rec;    // (sequence, tile of the sequence, contributors, slot of the first), contributors 0: none
+  int4* rec;    // (first row, packed rows, contributors, 2 * kv head + which slot of the first), contributors 0: none
   float2* ml;
   float* num;
 };
@@ -131,19 +142,19 @@ __host__ __device__ inline TokenWork token_work(void* p, int ctas) {
   return w;
 }
 
-// One sequence's share of the line of steps.
+// One sequence's share of the line of steps: hk tiles of `steps` steps.
 struct SeqWork {
   int q0, n, len, first;  // first row, new rows, positions, first step's position
-  int steps, tiles;       // steps of a tile; tiles (row tiles x kv heads)
+  int steps;
 };
 template <int kPos>
-QORA_DEV SeqWork seq_work(const AttnArgs& a, int s, int rows_per_tile) {
+QORA_DEV SeqWork seq_work(const AttnArgs& a, int s) {
   SeqWork w;
   w.q0 = a.batch.q_start[s];
   const int q1 = a.batch.q_start[s + 1];
   w.len = a.batch.kv_len[s];
   w.n = q1 - w.q0;
-  w.first = w.steps = w.tiles = 0;
+  w.first = w.steps = 0;
   const long long cap = (long long)a.batch.table_stride * a.pg.page_size;
   if (w.q0 < 0 || q1 < w.q0 || q1 > a.batch.rows || w.n > a.max_q || w.len < 0 || w.len > cap) {
     if (a.status) *a.status = 5u;
@@ -151,22 +162,29 @@ QORA_DEV SeqWork seq_work(const AttnArgs& a, int s, int rows_per_tile) {
   }
   if (w.n == 0) return w;
   const int lo = a.window > 0 ? max(0, w.len - w.n + 1 - a.window) : 0;
-  w.first = lo / kPos * kPos;
+  w.first = lo & ~(kPos - 1);
   w.steps = max(1, (w.len - w.first + kPos - 1) / kPos);
-  w.tiles = (w.n * a.group + rows_per_tile - 1) / rows_per_tile * a.hk;
   return w;
 }
 
+// CTA c's run of `total` steps over `ctas` CTAs: equal shares, the first ones a step longer.
+struct Share {
+  unsigned quot, rem;
+  QORA_DEV Share(unsigned total, unsigned ctas) : quot(total / ctas), rem(total % ctas) {}
+  QORA_DEV unsigned begin(unsigned c) const { return c * quot + min(c, rem); }
+  QORA_DEV unsigned owner(unsigned step) const {
+    const unsigned big = rem * (quot + 1);
+    return step < big ? step / (quot + 1) : rem + (step - big) / quot;
+  }
+};
+
 template <typename T, typename C, int D>
-__global__ void __launch_bounds__(32 * TokenCfg<T, C, D>::kWarps, 1) token_kernel(const AttnArgs a, void* work, int min_steps) {
+__global__ void __launch_bounds__(32 * TokenCfg<T, C, D>::kWarps, 1) token_kernel(const AttnArgs a, void* work, int min_steps, int tile_cost) {
   using Cfg = TokenCfg<T, C, D>;
   constexpr int kPos = Cfg::kPos, kRows = Cfg::kRows, kWarps = Cfg::kWarps, kChunks = Cfg::kChunks, kStages = Cfg::kStages;
   constexpr bool kWide = Cfg::kWide, kHalves = Cfg::kHalves;
   constexpr int kThr = 32 * kWarps;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ long long s_scan[kWarps];
-  __shared__ long long s_total, s_base;
-  __shared__ int s_seq;
   __shared__ float2 s_ml[kWarps][kRows];
   __shared__ uint32_t s_bad[kWarps][kStages];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -174,81 +192,80 @@ __global__ void __launch_bounds__(32 * TokenCfg<T, C, D>::kWarps, 1) token_kerne
   const TokenWork ws = token_work(work, gridDim.x);
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
-  // ---- this CTA's run of the line
-  long long mine = 0;
-  for (int s = tid; s < a.batch.seqs; s += kThr) {
-    const SeqWork w = seq_work<kPos>(a, s, kRows);
-    mine += (long long)w.steps * w.tiles;
-  }
-  for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-  if (lane == 0) s_scan[warp] = mine;
-  __syncthreads();
-  if (tid == 0) {
-    long long x = 0;
-    for (int w = 0; w < kWarps; ++w) x += s_scan[w];
-    s_total = x;
-    s_seq = a.batch.seqs;
-  }
-  __syncthreads();
-  const long long total = s_total;
-  // no more CTAs than leave min_steps each: a smaller share costs more to join than it saves
-  const long long ctas = max(1LL, min((long long)gridDim.x, (total + min_steps - 1) / min_steps));
-  const long long c = blockIdx.x;
+  // ---- this CTA's run of the line. Every warp scans the sequences' steps for itself (a lane
+  // holds a run of neighbouring sequences): no barrier, and the loads are in flight together
+  const unsigned c = blockIdx.x;
   if (tid == 0) ws.rec[c] = make_int4(0, 0, 0, 0);
-  if (c >= ctas) return;
-  long long cur = c * total / ctas;
-  const long long end = (c + 1) * total / ctas;
-  if (cur >= end) return;
-  {  // the sequence that holds step `cur`: scan in chunks of the CTA's threads
-    long long base = 0;
-    for (int s0 = 0; s0 < a.batch.seqs; s0 += kThr) {
-      const int s = s0 + tid;
-      long long v = 0;
-      if (s < a.batch.seqs) {
-        const SeqWork w = seq_work<kPos>(a, s, kRows);
-        v = (long long)w.steps * w.tiles;
-      }
-      long long x = v;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const long long y = __shfl_up_sync(0xffffffffu, x, o);
-        if (lane >= o) x += y;
-      }
-      if (lane == 31) s_scan[warp] = x;
-      __syncthreads();
-      long long before = base;
-      for (int w = 0; w < warp; ++w) before += s_scan[w];
-      long long all = base;
-      for (int w = 0; w < kWarps; ++w) all += s_scan[w];
-      if (v > 0 && before + x - v <= cur && cur < before + x) {
-        s_seq = s;
-        s_base = before + x - v;
-      }
-      __syncthreads();
-      base = all;
-      if (cur < base) break;
+  const int per = (a.batch.seqs + 31) >> 5;
+  unsigned mine = 0;
+  bool fits = true;
+#pragma unroll 4
+  for (int j = 0; j < per; ++j) {
+    const int s = lane * per + j;
+    if (s < a.batch.seqs) {
+      const SeqWork w = seq_work<kPos>(a, s);
+      const unsigned long long v = w.steps ? (unsigned long long)(w.steps + tile_cost) * (unsigned)a.hk : 0ull;
+      fits = fits && v < (1u << 26) && mine < (1u << 26);
+      mine += (unsigned)v;
     }
   }
-  int seq = s_seq;
-  long long base = s_base;
-  SeqWork sw = seq_work<kPos>(a, seq, kRows);
-  const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem + warp * Cfg::kRing);
+  fits = fits && mine < (1u << 26);  // 32 lanes: below 2^31
+  unsigned x = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const unsigned y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  const unsigned total = __shfl_sync(0xffffffffu, x, 31);
+  if (!__all_sync(0xffffffffu, fits)) {
+    if (tid == 0 && a.status) *a.status = 5u;
+    return;
+  }
+  if (total == 0) return;
+  // no more CTAs than leave min_steps each: a smaller share costs more to join than it saves
+  const unsigned ctas = min(gridDim.x, (total + min_steps - 1) / min_steps);
+  if (c >= ctas) return;
+  const Share share(total, ctas);
+  unsigned cur = share.begin(c);
+  const unsigned end = share.begin(c + 1);
+  int seq = lane * per;
+  unsigned base = x - mine;
+  const bool here = base <= cur && cur < x;
+  if (here) {
+    for (; seq + 1 < min(a.batch.seqs, (lane + 1) * per); ++seq) {
+      const SeqWork w = seq_work<kPos>(a, seq);
+      const unsigned v = w.steps ? (unsigned)(w.steps + tile_cost) * a.hk : 0u;
+      if (cur < base + v) break;
+      base += v;
+    }
+  }
+  const int src = __ffs(__ballot_sync(0xffffffffu, here)) - 1;
+  seq = __shfl_sync(0xffffffffu, seq, src);
+  base = __shfl_sync(0xffffffffu, base, src);
+  SeqWork sw = seq_work<kPos>(a, seq);
+  uint8_t* const ring = smem + warp * Cfg::kRing;
   const float scale2 = a.scale * kLog2e;
   const bool pow2 = (a.pg.page_size & (a.pg.page_size - 1)) == 0;
   const int shift = 31 - __clz(a.pg.page_size);
   bool first_seg = true;
+  int careful = 0;
 
   while (cur < end) {
-    while (cur >= base + (long long)sw.steps * sw.tiles) {  // the next sequence with work
-      base += (long long)sw.steps * sw.tiles;
+    for (unsigned v; cur - base >= (v = sw.steps ? (unsigned)(sw.steps + tile_cost) * a.hk : 0u);) {  // the next sequence with work
+      base += v;
       if (++seq >= a.batch.seqs) return;
-      sw = seq_work<kPos>(a, seq, kRows);
+      sw = seq_work<kPos>(a, seq);
     }
-    const long long in = cur - base;
-    const int tile = (int)(in / sw.steps), st0 = (int)(in % sw.steps);
-    const int st1 = (int)min((long long)sw.steps, st0 + (end - cur));
-    const int head = tile % a.hk, row0 = tile / a.hk * kRows;  // first packed row
-    const int nrows = min(kRows, sw.n * a.group - row0);
+    // units of the tile: tile_cost for the segment's fixed time, then its steps
+    const unsigned units = (unsigned)(sw.steps + tile_cost);
+    const int head = (int)((cur - base) / units);
+    const unsigned u0 = cur - base - (unsigned)head * units, u1 = min(units, u0 + (end - cur));
+    const int st0 = max(0, (int)u0 - tile_cost), st1 = max(0, (int)u1 - tile_cost);
+    if (st1 <= st0) {
+      cur += u1 - u0;
+      continue;
+    }
+    const int nrows = sw.n * a.group;
     const int p0 = sw.len - sw.n;
     const int* table = a.batch.table + (long long)seq * a.batch.table_stride;
     const C* kbase = static_cast<const C*>(a.k_pages) + head * a.pg.head_stride;
@@ -260,12 +277,11 @@ __global__ void __launch_bounds__(32 * TokenCfg<T, C, D>::kWarps, 1) token_kerne
     for (int i = 0; i < 2; ++i) {
       const int r = g + 8 * i;
       const bool ok = (!kHalves || i == 0) && r < nrows;
-      plast[i] = ok ? p0 + (row0 + r) / a.group : -1;
+      plast[i] = ok ? p0 + token_of(a, r) : -1;
       pfirst[i] = a.window > 0 ? max(0, plast[i] + 1 - a.window) : 0;
     }
-    const int seen_to = p0 + row0 / a.group;                       // every row sees up to here
-    const int top = p0 + (row0 + nrows - 1) / a.group;
-    const int seen_from = a.window > 0 ? max(0, top + 1 - a.window) : 0;  // and from here
+    // every row sees the positions from seen_from to p0
+    const int seen_from = a.window > 0 ? max(0, sw.len - a.window) : 0;
 
     // offset of position `pos` in the pages; -1: nothing there
     auto page_of = [&](int pos) -> int {
@@ -277,26 +293,25 @@ __global__ void __launch_bounds__(32 * TokenCfg<T, C, D>::kWarps, 1) token_kerne
       const int slot = pow2 ? pos & (a.pg.page_size - 1) : pos % a.pg.page_size;
       return page * a.pg.page_stride + (long long)slot * a.pg.slot_stride;
     };
+    const int crow = lane / kChunks, cch = lane % kChunks;  // the lane copies rows crow + i * (32 / kChunks), piece cch
     auto issue = [&](int step, int stage, int page) {  // page: of position step * kPos + lane
-      const int pos = sw.first + step * kPos + (lane & (kPos - 1));
-      const long long off = offset_of(pos, page);
-      const unsigned bad = __ballot_sync(0xffffffffu, off < 0 && lane < kPos);
+      constexpr int kHop = 32 / kChunks;
+      const int pos = sw.first + step * kPos;
+      const int left = sw.len - pos;  // positions that there are from here on
+      const uint32_t dk = ptx::smem_addr(ring + stage * Cfg::kStep), dv = dk + Cfg::kSide;
+      const unsigned gone = left >= kPos ? 0u : ~0u << max(0, left) & ((1u << kPos) - 1);
+      const long long off = offset_of(pos + (lane & (kPos - 1)), page);
+      const unsigned bad = __ballot_sync(0xffffffffu, off < 0) & ((1u << kPos) - 1);
+#pragma unroll
+      for (int i = 0; i < kPos / kHop; ++i) {
+        const long long o = __shfl_sync(0xffffffffu, off, crow + i * kHop);
+        const long long at = (o < 0 ? 0 : o) + cch * (16 / (int)sizeof(C));
+        cp_async_16(dk + Cfg::k_at(crow + i * kHop, cch), kbase + at, o >= 0);
+        cp_async_16(dv + Cfg::v_at(crow + i * kHop, cch), vbase + at, o >= 0);
+      }
       if (lane == 0) {
         s_bad[warp][stage] = bad;
-        if (a.status)  // a page that does not exist, unlike a slot behind the last position
-          for (unsigned b = bad; b; b &= b - 1)
-            if (pos + __ffs(b) - 1 < sw.len) *a.status = 5u;
-      }
-      const uint32_t dk = ring + stage * 2 * Cfg::kSide, dv = dk + Cfg::kSide;
-#pragma unroll
-      for (int i = 0; i < kPos * kChunks / 32; ++i) {
-        const int row = (i * 32) / kChunks + lane / kChunks, ch = lane % kChunks;
-        const long long o = __shfl_sync(0xffffffffu, off, row);
-        const long long at = (o < 0 ? 0 : o) + ch * (16 / (int)sizeof(C));
-        const int ck = kWide ? ch ^ ((row & 1) << 2) : ch ^ (row & 7);
-        const int cv = kWide ? ch ^ (row & 6) : ch ^ (row & 7);
-        cp_async_16(dk + (row * kChunks + ck) * 16, kbase + at, o >= 0);
-        cp_async_16(dv + (row * kChunks + cv) * 16, vbase + at, o >= 0);
+        if (a.status && (bad & ~gone)) *a.status = 5u;  // a page that does not exist
       }
     };
 
@@ -304,60 +319,64 @@ __global__ void __launch_bounds__(32 * TokenCfg<T, C, D>::kWarps, 1) token_kerne
     float qscale[2] = {scale2, scale2};
     constexpr int kQ = kWide ? D / 8 : D / 16;
     uint32_t qa[kQ][4];
-    auto load_q = [&]() {
-      auto row_ptr = [&](int r) {
-        const int pr = row0 + r;
-        return static_cast<const T*>(a.q) + (long long)(sw.q0 + pr / a.group) * a.q_stride + (head * a.group + pr % a.group) * D;
-      };
-      if constexpr (!kHalves) {
+    auto row_ptr = [&](int r) {
+      const int tok = token_of(a, r);
+      return static_cast<const T*>(a.q) + (long long)(sw.q0 + tok) * a.q_stride + (head * a.group + r - tok * a.group) * D;
+    };
+    float qx[kHalves ? 2 * D / 8 : 1];  // f32 rows as loaded; the loads are under way while the first copies are issued
+    if constexpr (!kHalves) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const bool ok = g + 8 * i < nrows;
-          const T* q = row_ptr(ok ? g + 8 * i : 0);
+      for (int i = 0; i < 2; ++i) {
+        const bool ok = g + 8 * i < nrows;
+        const T* q = row_ptr(ok ? g + 8 * i : 0);
 #pragma unroll
-          for (int k = 0; k < kQ; ++k) {
-            qa[k][i] = ok ? *reinterpret_cast<const uint32_t*>(q + 16 * k + 2 * t) : 0u;
-            qa[k][2 + i] = ok ? *reinterpret_cast<const uint32_t*>(q + 16 * k + 8 + 2 * t) : 0u;
-          }
+        for (int k = 0; k < kQ; ++k) {
+          qa[k][i] = ok ? *reinterpret_cast<const uint32_t*>(q + 16 * k + 2 * t) : 0u;
+          qa[k][2 + i] = ok ? *reinterpret_cast<const uint32_t*>(q + 16 * k + 8 + 2 * t) : 0u;
         }
-      } else {
-        const bool ok = g < nrows;
-        const float* q = reinterpret_cast<const float*>(row_ptr(ok ? g : 0));
+      }
+    } else {
+      const float* q = reinterpret_cast<const float*>(row_ptr(g < nrows ? g : 0));
+      constexpr int kV = kWide ? 4 : 2;  // floats of a load: 16 b + 4 t.. or 8 k + 2 t..
+#pragma unroll
+      for (int k = 0; k < D / 4 / kV; ++k)
+#pragma unroll
+        for (int j = 0; j < kV; j += 2) {
+          const float2 y = *reinterpret_cast<const float2*>(q + 4 * kV * k + kV * t + j);
+          qx[kV * k + j] = y.x;
+          qx[kV * k + j + 1] = y.y;
+        }
+    }
+    auto make_q = [&]() {
+      if constexpr (kHalves) {
+        if (g >= nrows) {
+#pragma unroll
+          for (int k = 0; k < D / 4; ++k) qx[k] = 0.0f;
+        }
         if constexpr (kWide) {  // tf32: the exponent range is f32's, no scale
 #pragma unroll
-          for (int b = 0; b < D / 16; ++b) {
-            float4 x = *reinterpret_cast<const float4*>(q + 16 * b + 4 * t);
-            if (!ok) x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            const float e[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              qa[2 * b + (j >> 1)][2 * (j & 1)] = tf32_hi(e[j]);
-              qa[2 * b + (j >> 1)][2 * (j & 1) + 1] = tf32_lo(e[j]);
-            }
+          for (int k = 0; k < D / 4; ++k) {
+            qa[k >> 1][2 * (k & 1)] = tf32_hi(qx[k]);
+            qa[k >> 1][2 * (k & 1) + 1] = tf32_lo(qx[k]);
           }
         } else {
-          float2 x[2 * kQ];
           float mx = 0.0f;
 #pragma unroll
-          for (int k = 0; k < 2 * kQ; ++k) {
-            x[k] = *reinterpret_cast<const float2*>(q + 8 * k + 2 * t);
-            if (!ok) x[k] = make_float2(0.0f, 0.0f);
-            mx = fmaxf(mx, fmaxf(fabsf(x[k].x), fabsf(x[k].y)));
-          }
+          for (int k = 0; k < D / 4; ++k) mx = fmaxf(mx, fabsf(qx[k]));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
           // exponent of mx (0 for zeros and subnormals, 255 for non-finite rows: no scale)
           const int ex = (int)(__float_as_uint(mx) >> 23);
-          const int up = ex == 0 || ex == 255 ? 0 : min(127, max(-126, 140 - ex));
+          const int up = ex == 0 || ex == 255 ? 0 : min(126, 140 - ex);
           const float mul = __uint_as_float((uint32_t)(127 + up) << 23);
-          qscale[0] = scale2 * __uint_as_float((uint32_t)(127 - (up == 127 ? 126 : up)) << 23) * (up == 127 ? 0.5f : 1.0f);
+          qscale[0] = scale2 * __uint_as_float((uint32_t)(127 - up) << 23);
 #pragma unroll
-          for (int k = 0; k < 2 * kQ; ++k) {
-            const float u = x[k].x * mul, v = x[k].y * mul;
+          for (int k = 0; k < D / 8; ++k) {
+            const float u = qx[2 * k] * mul, v = qx[2 * k + 1] * mul;
             const uint32_t hi = pack2(u, v, __half());
             const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&hi));
-            qa[k / 2][2 * (k & 1)] = hi;
-            qa[k / 2][2 * (k & 1) + 1] = pack2(u - h.x, v - h.y, __half());
+            qa[k >> 1][2 * (k & 1)] = hi;
+            qa[k >> 1][2 * (k & 1) + 1] = pack2(u - h.x, v - h.y, __half());
           }
         }
       }
@@ -366,8 +385,7 @@ __global__ void __launch_bounds__(32 * TokenCfg<T, C, D>::kWarps, 1) token_kerne
     constexpr int kO = D / 8;  // numerators: n8 tiles of 4 values
     float o[kO][4];
     float m[2], l[2];
-    bool q_loaded = false;
-    for (int careful = 0; careful < 2; ++careful) {
+    {
 #pragma unroll
       for (int i = 0; i < kO; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
       m[0] = m[1] = -INFINITY;
@@ -375,33 +393,29 @@ __global__ void __launch_bounds__(32 * TokenCfg<T, C, D>::kWarps, 1) token_kerne
       const int nst = st1 - st0 > warp ? (st1 - st0 - warp + kWarps - 1) / kWarps : 0;  // this warp's steps
       const int my0 = st0 + warp;
       auto next_page = [&](int i) { return i < nst ? page_of(sw.first + (my0 + i * kWarps) * kPos + (lane & (kPos - 1))) : -1; };
-      int page = next_page(0);
-#pragma unroll
-      for (int i = 0; i < kStages - 1; ++i) {
-        const int np = next_page(i + 1);
-        if (i < nst) issue(my0 + i * kWarps, i, page);
+      int page = next_page(0), stage = 0, fill = 0;
+#pragma unroll 1
+      for (int i = 1 - kStages; i < nst; ++i) {
+        if (i >= 0) cp_async_wait<kStages - 2>();
+        __syncwarp();
+        const int np = next_page(i + kStages);
+        if (i + kStages - 1 < nst) issue(my0 + (i + kStages - 1) * kWarps, fill, page);  // into the stage that the previous step left
         cp_async_commit();
         page = np;
-      }
-      if (!q_loaded) load_q();
-      q_loaded = true;
-      int stage = 0;
-      for (int i = 0; i < nst; ++i) {
-        cp_async_wait<kStages - 2>();
-        __syncwarp();
-        {  // refill the stage that the previous step left
-          const int ns = stage == 0 ? kStages - 1 : stage - 1;
-          const int np = next_page(i + kStages);
-          if (i + kStages - 1 < nst) issue(my0 + (i + kStages - 1) * kWarps, ns, page);
-          cp_async_commit();
-          page = np;
+        fill = fill + 1 == kStages ? 0 : fill + 1;
+        if (i < 0) {
+          if (i == -1) make_q();
+          continue;
         }
         const int pos0 = sw.first + (my0 + i * kWarps) * kPos;
-        const uint32_t sk = ring + stage * 2 * Cfg::kSide, sv = sk + Cfg::kSide;
+        uint8_t* const pk = ring + stage * Cfg::kStep;
+        uint8_t* const pv = pk + Cfg::kSide;
+        const uint32_t sk = ptx::smem_addr(pk), sv = ptx::smem_addr(pv);
         const uint32_t bad = s_bad[warp][stage];
         if (careful) {  // non-finite elements of V become zero
+#pragma unroll 1
           for (int x = lane; x < kPos * kChunks; x += 32) {
-            uint4* p = reinterpret_cast<uint4*>(smem + warp * Cfg::kRing + stage * 2 * Cfg::kSide + Cfg::kSide) + x;
+            uint4* p = reinterpret_cast<uint4*>(pv) + x;
             uint4 v = *p;
             C* e = reinterpret_cast<C*>(&v);
             for (int y = 0; y < 16 / (int)sizeof(C); ++y)
@@ -417,8 +431,7 @@ __global__ void __launch_bounds__(32 * TokenCfg<T, C, D>::kWarps, 1) token_kerne
           float u[4] = {0.0f, 0.0f, 0.0f, 0.0f}, v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
           for (int b = 0; b < D / 16; ++b) {
-            const int ch = (4 * b + t) ^ ((g & 1) << 2);
-            const float4 k = *reinterpret_cast<const float4*>(smem + warp * Cfg::kRing + stage * 2 * Cfg::kSide + (g * kChunks + ch) * 16);
+            const float4 k = *reinterpret_cast<const float4*>(pk + Cfg::k_at(g, 4 * b + t));
             mma_tf32(u, qa[2 * b], tf32_hi(k.x), tf32_hi(k.y));
             mma_tf32(v, qa[2 * b], tf32_lo(k.x), tf32_lo(k.y));
             mma_tf32(u, qa[2 * b + 1], tf32_hi(k.z), tf32_hi(k.w));
@@ -433,7 +446,7 @@ __global__ void __launch_bounds__(32 * TokenCfg<T, C, D>::kWarps, 1) token_kerne
 #pragma unroll
           for (int k = 0; k < kQ; ++k) {
             uint32_t b[4];
-            ldsm4(b, sk + (row * kChunks + ((2 * k + (mi & 1)) ^ (row & 7))) * 16);
+            ldsm4(b, sk + Cfg::k_at(row, 2 * k + (mi & 1)));
             mma16(s[0], qa[k], b[0], b[1], C());
             mma16(s[1], qa[k], b[2], b[3], C());
           }
@@ -446,7 +459,7 @@ __global__ void __launch_bounds__(32 * TokenCfg<T, C, D>::kWarps, 1) token_kerne
             s[n][1] += s[n][3];
           }
         }
-        const bool plain = pos0 >= seen_from && pos0 + kPos - 1 <= seen_to && bad == 0;
+        const bool plain = pos0 >= seen_from && pos0 + kPos - 1 <= p0 && bad == 0;
         float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
         for (int n = 0; n < kN; ++n)
@@ -504,10 +517,8 @@ __global__ void __launch_bounds__(32 * TokenCfg<T, C, D>::kWarps, 1) token_kerne
           const uint32_t pa[4] = {tf32_hi(s[0][0]), tf32_lo(s[0][0]), tf32_hi(s[0][1]), tf32_lo(s[0][1])};
 #pragma unroll
           for (int b = 0; b < D / 32; ++b) {
-            const uint8_t* vp = smem + warp * Cfg::kRing + stage * 2 * Cfg::kSide + Cfg::kSide;
-            const int ch = 8 * b + g;
-            const float4 v0 = *reinterpret_cast<const float4*>(vp + ((2 * t) * kChunks + (ch ^ ((2 * t) & 6))) * 16);
-            const float4 v1 = *reinterpret_cast<const float4*>(vp + ((2 * t + 1) * kChunks + (ch ^ ((2 * t + 1) & 6))) * 16);
+            const float4 v0 = *reinterpret_cast<const float4*>(pv + Cfg::v_at(2 * t, 8 * b + g));
+            const float4 v1 = *reinterpret_cast<const float4*>(pv + Cfg::v_at(2 * t + 1, 8 * b + g));
             const float e0[4] = {v0.x, v0.y, v0.z, v0.w}, e1[4] = {v1.x, v1.y, v1.z, v1.w};
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -539,7 +550,7 @@ __global__ void __launch_bounds__(32 * TokenCfg<T, C, D>::kWarps, 1) token_kerne
 #pragma unroll
           for (int d = 0; d < D / 16; ++d) {
             uint32_t b[4];
-            ldsm4_t(b, sv + (row * kChunks + ((2 * d + (mi >> 1)) ^ (row & 7))) * 16);
+            ldsm4_t(b, sv + Cfg::v_at(row, 2 * d + (mi >> 1)));
             if constexpr (kHalves) {
               float acc[2][4] = {};
               mma16(acc[0], pa, b[0], b[1], C());
@@ -561,7 +572,9 @@ __global__ void __launch_bounds__(32 * TokenCfg<T, C, D>::kWarps, 1) token_kerne
       cp_async_wait<0>();
       __syncwarp();
       if (careful) {  // the non-finite elements, for the rows that see them
+#pragma unroll 1
         for (int i = 0; i < nst; ++i)
+#pragma unroll 1
           for (int w = 0; w < kPos; ++w) {
             const int pos = sw.first + (my0 + i * kWarps) * kPos + w;
             const long long off = offset_of(pos, page_of(pos));
@@ -577,14 +590,7 @@ __global__ void __launch_bounds__(32 * TokenCfg<T, C, D>::kWarps, 1) token_kerne
                 if (!kHalves && pos <= plast[1] && pos >= pfirst[1]) o[x][2 + j] += v;
               }
           }
-        break;
       }
-      float z = 0.0f;
-#pragma unroll
-      for (int x = 0; x < kO; ++x)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) z = __fmaf_rn(o[x][j], 0.0f, z);
-      if (!__any_sync(0xffffffffu, z != 0.0f)) break;  // z is 0, or NaN where a numerator is not finite
     }
 
     // ---- the warps' shares of the segment, in warp order
@@ -595,21 +601,37 @@ __global__ void __launch_bounds__(32 * TokenCfg<T, C, D>::kWarps, 1) token_kerne
       if (t == 0) s_ml[warp][g + 8 * r] = make_float2(m[r], l[r]);
     }
     {
-      float* dst = reinterpret_cast<float*>(smem + warp * Cfg::kRing);
+      float* dst = reinterpret_cast<float*>(ring) + g * Cfg::kNum;
+      if constexpr (kWide) {
 #pragma unroll
-      for (int x = 0; x < kO; ++x)
+        for (int b = 0; b < D / 32; ++b)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int dim = kWide ? 32 * (x >> 2) + 4 * (2 * t + j) + (x & 3) : 8 * x + 2 * t + j;
+          for (int j = 0; j < 2; ++j)
+            *reinterpret_cast<float4*>(dst + 32 * b + 4 * (2 * t + j)) =
+                make_float4(o[4 * b][j] + o[4 * b][2 + j], o[4 * b + 1][j] + o[4 * b + 1][2 + j],
+                            o[4 * b + 2][j] + o[4 * b + 2][2 + j], o[4 * b + 3][j] + o[4 * b + 3][2 + j]);
+      } else {
+#pragma unroll
+        for (int x = 0; x < kO; ++x) {
           if constexpr (kHalves) {
-            dst[g * D + dim] = o[x][j] + o[x][2 + j];
+            *reinterpret_cast<float2*>(dst + 8 * x + 2 * t) = make_float2(o[x][0] + o[x][2], o[x][1] + o[x][3]);
           } else {
-            dst[g * D + dim] = o[x][j];
-            dst[(g + 8) * D + dim] = o[x][2 + j];
+            *reinterpret_cast<float2*>(dst + 8 * x + 2 * t) = make_float2(o[x][0], o[x][1]);
+            *reinterpret_cast<float2*>(dst + 8 * Cfg::kNum + 8 * x + 2 * t) = make_float2(o[x][2], o[x][3]);
           }
         }
+      }
     }
-    __syncthreads();
+    float z = 0.0f;  // 0, or NaN where a numerator is not finite
+#pragma unroll
+    for (int x = 0; x < kO; ++x)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) z = __fmaf_rn(o[x][j], 0.0f, z);
+    if (__syncthreads_or(z != 0.0f) && !careful) {
+      careful = 1;
+      continue;
+    }
+    careful = 0;
     const bool whole = st0 == 0 && st1 == sw.steps;
     const int slot = 2 * (int)c + (first_seg ? 0 : 1);
     for (int x = tid; x < nrows * (D / 4); x += kThr) {
@@ -622,7 +644,7 @@ __global__ void __launch_bounds__(32 * TokenCfg<T, C, D>::kWarps, 1) token_kerne
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
         const float f = exp2_approx(s_ml[w][r].x - mu);
-        const float4 y = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(smem + w * Cfg::kRing) + r * D + d);
+        const float4 y = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(smem + w * Cfg::kRing) + r * Cfg::kNum + d);
         ll = __fmaf_rn(s_ml[w][r].y, f, ll);
         v[0] = __fmaf_rn(y.x, f, v[0]);
         v[1] = __fmaf_rn(y.y, f, v[1]);
@@ -633,7 +655,7 @@ __global__ void __launch_bounds__(32 * TokenCfg<T, C, D>::kWarps, 1) token_kerne
         const float inv = ll == 0.0f ? 0.0f : __fdiv_rn(1.0f, ll);
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[j] *= inv;
-        const int pr = row0 + r, row = sw.q0 + pr / a.group, h = head * a.group + pr % a.group;
+        const int tok = token_of(a, r), row = sw.q0 + tok, h = head * a.group + r - tok * a.group;
         store_elems(static_cast<T*>(a.out) + (long long)row * a.out_stride + h * D + d, v);
         if (a.lse && d == 0)
           a.lse[(long long)row * a.hq + h] = ll == 0.0f ? -INFINITY : (mm - kShift + log2f(ll)) * kLn2;
@@ -643,21 +665,18 @@ __global__ void __launch_bounds__(32 * TokenCfg<T, C, D>::kWarps, 1) token_kerne
       }
     }
     if (!whole && st0 == 0 && tid == 0) {  // a cut tile begins here: its last step's CTA is the last contributor
-      const long long last = cur + sw.steps - 1;
-      long long e = last * ctas / total;
-      while ((e + 1) * total / ctas <= last) ++e;
-      while (e * total / ctas > last) --e;
-      ws.rec[c] = make_int4(seq, tile, (int)(e - c) + 1, slot);
+      const unsigned e = share.owner(base + (unsigned)(head + 1) * units - 1);
+      ws.rec[c] = make_int4(sw.q0, sw.n * a.group, (int)(e - c) + 1, 2 * head + (first_seg ? 0 : 1));
     }
     __syncthreads();
-    cur += st1 - st0;
+    cur += u1 - u0;
     first_seg = false;
   }
 }
 
 // The cut tiles: block (c, r) joins row r of the tile whose first part CTA c holds, in CTA
 // order. Four warps take every fourth contributor.
-template <typename T, int D, int kRows>
+template <typename T, int D>
 __global__ void __launch_bounds__(128) token_join_kernel(const AttnArgs a, void* work, int ctas) {
   __shared__ float s_w[kTokenMaxCtas];
   __shared__ float s_o[4][D];
@@ -667,36 +686,60 @@ __global__ void __launch_bounds__(128) token_join_kernel(const AttnArgs a, void*
   const int c = blockIdx.x, r = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int4 rec = ws.rec[c];
   const int count = rec.z;
-  if (count == 0) return;
-  const int q0 = a.batch.q_start[rec.x], n = a.batch.q_start[rec.x + 1] - q0;
-  const int head = rec.y % a.hk, pr = rec.y / a.hk * kRows + r;
-  if (pr >= n * a.group) return;
-  auto slot_of = [&](int i) -> size_t { return ((size_t)(i == 0 ? rec.w : 2 * (c + i)) * kTokenMaxRows + r); };
+  if (r >= rec.y || count == 0) return;
+  const int head = rec.w >> 1;
+  auto slot_of = [&](int i) -> size_t { return (size_t)(2 * (c + i) + (i == 0 ? rec.w & 1 : 0)) * kTokenMaxRows + r; };
+  // the first contributors' numerators are on their way while the weights are found
+  constexpr int E = D / 32, kAhead = 10;
+  float y[kAhead][E];
+#pragma unroll
+  for (int k = 0; k < kAhead; ++k) {
+    const int i = warp + 4 * k;
+    const float* p = ws.num + slot_of(i < count ? i : 0) * D + lane * E;
+#pragma unroll
+    for (int j = 0; j < E; j += 2) {
+      const float2 v = *reinterpret_cast<const float2*>(p + j);
+      y[k][j] = v.x;
+      y[k][j + 1] = v.y;
+    }
+  }
+  float2 ml[(kTokenMaxCtas + 127) / 128];
   float mm = -INFINITY;
-  for (int i = tid; i < count; i += 128) mm = fmaxf(mm, ws.ml[slot_of(i)].x);
+#pragma unroll
+  for (int k = 0; k < (kTokenMaxCtas + 127) / 128; ++k) {
+    const int i = tid + 128 * k;
+    ml[k] = i < count ? ws.ml[slot_of(i)] : make_float2(-INFINITY, 0.0f);
+    mm = fmaxf(mm, ml[k].x);
+  }
   mm = warp_max(mm);
   if (lane == 0) s_red[warp] = mm;
   __syncthreads();
   mm = fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3]));
   const float mu = mm == -INFINITY ? 0.0f : mm;
   float ll = 0.0f;
-  __syncthreads();
-  for (int i = tid; i < count; i += 128) {
-    const float2 x = ws.ml[slot_of(i)];
-    const float f = exp2_approx(x.x - mu);
-    s_w[i] = f;
-    ll = __fmaf_rn(x.y, f, ll);
+#pragma unroll
+  for (int k = 0; k < (kTokenMaxCtas + 127) / 128; ++k) {
+    const int i = tid + 128 * k;
+    const float f = exp2_approx(ml[k].x - mu);
+    if (i < count) s_w[i] = f;
+    ll = __fmaf_rn(ml[k].y, f, ll);
   }
   ll = warp_sum(ll);
+  __syncthreads();  // s_red is read by all before it is written again
   if (lane == 0) s_red[warp] = ll;
   __syncthreads();
   ll = (s_red[0] + s_red[1]) + (s_red[2] + s_red[3]);
-  constexpr int E = D / 32;
   float v[E];
 #pragma unroll
   for (int j = 0; j < E; ++j) v[j] = 0.0f;
-#pragma unroll 8
-  for (int i = warp; i < count; i += 4) {
+#pragma unroll
+  for (int k = 0; k < kAhead; ++k)
+    if (warp + 4 * k < count) {
+#pragma unroll
+      for (int j = 0; j < E; ++j) v[j] = __fmaf_rn(y[k][j], s_w[warp + 4 * k], v[j]);
+    }
+#pragma unroll 4
+  for (int i = warp + 4 * kAhead; i < count; i += 4) {
     const float* p = ws.num + slot_of(i) * D + lane * E;
     const float f = s_w[i];
 #pragma unroll
@@ -705,7 +748,7 @@ __global__ void __launch_bounds__(128) token_join_kernel(const AttnArgs a, void*
 #pragma unroll
   for (int j = 0; j < E; ++j) s_o[warp][lane * E + j] = v[j];
   __syncthreads();
-  const int row = q0 + pr / a.group, h = head * a.group + pr % a.group;
+  const int tok = token_of(a, r), row = rec.x + tok, h = head * a.group + r - tok * a.group;
   if (tid < D) {
     const float x = ((s_o[0][tid] + s_o[1][tid]) + s_o[2][tid]) + s_o[3][tid];
     static_cast<T*>(a.out)[(long long)row * a.out_stride + h * D + tid] = from_f32(ll == 0.0f ? 0.0f : __fmul_rn(x, __fdiv_rn(1.0f, ll)), T());
