@@ -10,6 +10,7 @@
 
 #include "host_util.h"
 #include "paged_attention.cuh"
+#include "paged_chunk.cuh"
 #include "paged_rows.cuh"
 #include "paged_token.cuh"
 
@@ -159,8 +160,39 @@ qora_status launch_token(const paged::AttnArgs& a, void* work, cudaStream_t s) {
 }
 
 template <typename T, typename C, int D>
+qora_status launch_chunk(const paged::AttnArgs& a, void* work, cudaStream_t s) {
+  using Cfg = paged::ChunkCfg<T, C, D>;
+  int dev = 0;
+  QCUDA(cudaGetDevice(&dev));
+  QCHECK((allow_smem<&paged::chunk_kernel<T, C, D>>(dev, Cfg::kSmem)));
+  const int sms = std::min(sm_count(dev), paged::kChunkMaxCtas);
+  const int tokens = Cfg::kRows / a.group;
+  // row tiles that sequences with disjoint rows can have; items of long caches are split
+  // until there is one for every SM
+  const long long most = ((long long)a.batch.rows + (long long)a.batch.seqs * (tokens - 1)) / tokens * a.hk;
+  if (most > 0x7fffffff / sms) return fail(QORA_ERR_INVALID, "%d rows of %d sequences", a.batch.rows, a.batch.seqs);
+  const int splits = most >= sms ? 1 : (int)(sms / most);
+  const int ctas = (int)std::min<long long>(sms, most * splits);
+  paged::chunk_kernel<T, C, D><<<ctas, Cfg::kThreads, Cfg::kSmem, s>>>(a, work, tokens, splits, (int)(most * splits));
+  QCUDA(cudaGetLastError());
+  if (splits == 1) return QORA_OK;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)most, std::min(Cfg::kRows, (int)std::min<long long>(a.max_q, tokens) * a.group + 7) / 8);
+  cfg.blockDim = dim3(256);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  QCUDA(cudaLaunchKernelEx(&cfg, paged::chunk_join_kernel<T, D>, a, work, tokens, splits));
+  return QORA_OK;
+}
+
+template <typename T, typename C, int D>
 qora_status launch_attn(const paged::AttnArgs& a, void* work, cudaStream_t s) {
   if ((long long)a.max_q * a.group <= paged::TokenCfg<T, C, D>::kRows) return launch_token<T, C, D>(a, work, s);
+  if constexpr (sizeof(C) == 2) return launch_chunk<T, C, D>(a, work, s);
   const long long units = (long long)a.batch.rows * a.hq;
   paged::attn_row_kernel<T, C, D><<<(unsigned)((units + 7) / 8), 256, 0, s>>>(a);
   QCUDA(cudaGetLastError());
