@@ -10,13 +10,16 @@
 // parts in order. Items are taken from the last rows (the longest runs of positions) on, in
 // alternating direction, so the CTAs end together.
 //
-// Roles (512 threads, one CTA per SM):
+// Roles (384 threads, one CTA per SM: a softmax thread keeps its row's 128 scores in registers):
 //   warps 0-3, 4-7   softmax of block 0, 1: a thread owns a row, reads its 128 scores from
 //                    TMEM, writes the weights back over them as the next product's operand
-//   warps 8-11       loads: pages are looked up per position and copied by cp.async in 16-byte
-//                    pieces (any page size and stride; slots past the end become zeros) into
-//                    the 128-byte-swizzled tiles that the products read
-//   warp 12          issues the products: S_X = Q_X K^T; O_X += P_X V with P_X from TMEM
+//   warp 8           issues the products: S_X = Q_X K^T; O_X += P_X V with P_X from TMEM
+//   warps 9, 10      load K and V into the 128-byte-swizzled tiles that the products read. A
+//                    tile whose 128 positions all exist comes by TMA, a page (or 128 rows of
+//                    one) per copy, where the page size divides 128 or is a multiple of it;
+//                    other tiles are copied by cp.async in 16-byte pieces, the page looked up
+//                    per position (slots past the end become zeros)
+//   warp 11          loads q (f32 rows: warps 9-11, which split it)
 // While one block's weights are computed the other block's products run. S_X(j + 1) is
 // issued behind O_X(j), which still reads P_X(j) from the columns it overwrites: one
 // thread's products execute in order.
@@ -31,6 +34,8 @@
 // infinite value of V, or a row whose own scores are) is computed again by one warp, one
 // position at a time (row_attend).
 #pragma once
+
+#include <cuda.h>
 
 #include <type_traits>
 
@@ -57,7 +62,8 @@ struct ChunkCfg {
   static_assert(kStages >= 3, "a K tile, a V tile and the next K tile");
   static constexpr int kLag = kStages >= 4 ? 2 : 1;  // copies in flight behind the newest: at most kStages - 2
   static constexpr int kSmem = kQBytes + kStages * kStage + kOther + 1024;
-  static constexpr int kThreads = 512;
+  static constexpr int kThreads = 384;
+  static constexpr int kLoaders = 64;
 };
 constexpr int kChunkMaxCtas = 160;
 constexpr unsigned long long kWaitNs = 2000000000ull;
@@ -91,27 +97,57 @@ QORA_DEV void tmem_st32(uint32_t taddr, const uint32_t* r) {
       "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr)
       : "memory");
 }
-QORA_DEV void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-
-// D[tmem] (+)= A[tmem] . B[smem], kind::f16
-QORA_DEV void mma_ts(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+// box at (x, slot, head, page) of the pages to shared memory, completing on `bar`
+QORA_DEV void tma_4d(uint32_t dst, const CUtensorMap* map, int x, int slot, int head, int page, uint64_t* bar) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
-      "r"(a), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(
+          dst),
+      "l"(map), "r"(x), "r"(slot), "r"(head), "r"(page), "r"(ptx::smem_addr(bar))
       : "memory");
 }
+QORA_DEV void tmem_ld16(uint32_t taddr, float* v) {
+  uint32_t* r = reinterpret_cast<uint32_t*>(v);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+QORA_DEV void tmem_st16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(r[0]),
+      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
+      : "memory");
+}
+QORA_DEV void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // Tiles are [rows][64 elements] halves of 128-byte rows, 16-byte pieces permuted by the row
 // (128-byte swizzle; 8-row groups 1024 bytes apart), the second half `rows * 128` bytes on.
 // Read K-major (k along the row): a k step of 16 is 32 bytes on. Read MN-major (k down the
 // rows): groups of 8 k are 1024 bytes apart, groups of 64 columns `rows * 128`.
-QORA_DEV uint64_t desc_k(uint32_t addr) {
-  return (uint64_t)((addr >> 4) & 0x3FFFu) | (1ull << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+// A matrix descriptor's upper word is the same for all; in the lower one the address counts
+// 16 bytes, so a step is one addition: the issuing thread has 64 cycles per product.
+constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+QORA_DEV uint32_t desc_k(uint32_t addr) { return ((addr >> 4) & 0x3FFFu) | (1u << 16); }
+QORA_DEV uint32_t desc_mn(uint32_t addr, uint32_t half) { return ((addr >> 4) & 0x3FFFu) | ((half >> 4) << 16); }
+
+// D[tmem] (+)= A[smem] . B[smem], kind::f16
+QORA_DEV void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n .reg .b64 da, db;\n mov.b64 da, {%1, %5};\n mov.b64 db, {%2, %5};\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n}\n" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "r"(kDescHi)
+      : "memory");
 }
-QORA_DEV uint64_t desc_mn(uint32_t addr, uint32_t half) {
-  return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)(half >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) |
-         (2ull << 61);
+// D[tmem] (+)= A[tmem] . B[smem], kind::f16
+QORA_DEV void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n .reg .b64 db;\n mov.b64 db, {%2, %5};\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n}\n" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "r"(kDescHi)
+      : "memory");
 }
 // f32 accumulators, M = 128, N = n; b_mn: B is MN-major
 template <typename C>
@@ -229,7 +265,9 @@ QORA_DEV void row_attend(const AttnArgs& a, const T* q, const int* table, int he
 }
 
 template <typename T, typename C, int D>
-__global__ void __launch_bounds__(512, 1) chunk_kernel(const AttnArgs a, void* work, int tokens, int splits, int max_items) {
+__global__ void __launch_bounds__(384, 1) chunk_kernel(const AttnArgs a, void* work, int tokens, int splits, int max_items, int box_rows,
+                                                       const __grid_constant__ CUtensorMap kmap,
+                                                       const __grid_constant__ CUtensorMap vmap) {
   using Cfg = ChunkCfg<T, C, D>;
   constexpr bool kHalves = Cfg::kHalves;
   constexpr int kPos = Cfg::kPos, kParts = Cfg::kParts, kStages = Cfg::kStages, kLag = Cfg::kLag;
@@ -251,10 +289,10 @@ __global__ void __launch_bounds__(512, 1) chunk_kernel(const AttnArgs a, void* w
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (tid == 0) {
     for (int i = 0; i < kStages; ++i) {
-      ptx::mbar_init(full + i, 128);
+      ptx::mbar_init(full + i, 1);
       ptx::mbar_init(empty + i, 1);
     }
-    ptx::mbar_init(q_full, 128);
+    ptx::mbar_init(q_full, kHalves ? 96 : 32);
     ptx::mbar_init(q_empty, 1);
     for (int x = 0; x < 2; ++x) {
       ptx::mbar_init(s_full + x, 1);
@@ -265,7 +303,7 @@ __global__ void __launch_bounds__(512, 1) chunk_kernel(const AttnArgs a, void* w
     *abort_flag = 0;
     ptx::fence_mbar_init();
   }
-  if (warp == 12) umma::tmem_alloc(s_tmem, 512);
+  if (warp == 8) umma::tmem_alloc(s_tmem, 512);
   umma::tc_fence_before();
   __syncthreads();
   umma::tc_fence_after();
@@ -282,11 +320,13 @@ __global__ void __launch_bounds__(512, 1) chunk_kernel(const AttnArgs a, void* w
   auto item_of = [&](int w) { return w * ctas + (w & 1 ? ctas - 1 - cta : cta); };
   auto wait = [&](uint64_t* bar, uint32_t parity) { return umma::wait_bar(bar, parity, kWaitNs, abort_flag); };
 
-  if (warp >= 12) {
-    if (warp == 12) {
+  if (warp == 8) {
+    {
       // ---------------------------------------------------------------- products
       uint32_t tile = 0, turn = 0, ns_done[2] = {0, 0};
       bool ok = true;
+      const uint32_t q_k = desc_k(ptx::smem_addr(sq)), ring_k = desc_k(ptx::smem_addr(ring)),
+                     ring_mn = desc_mn(ptx::smem_addr(ring), kHalfKV);
       constexpr uint32_t id_s = chunk_idesc<C>(kPos, false), id_o = chunk_idesc<C>(D, true);
       for (int w = 0; ok && w * ctas < items; ++w) {
         const int idx = item_of(w);
@@ -298,15 +338,14 @@ __global__ void __launch_bounds__(512, 1) chunk_kernel(const AttnArgs a, void* w
           // ring entries alternate K, V: entry e lies in stage e % kStages
           auto entry = [&](uint32_t e) { return wait(full + e % kStages, (e / kStages) & 1); };
           auto scores = [&](int x, uint32_t e) {
-            const uint32_t kb = ptx::smem_addr(ring + (e % kStages) * Cfg::kStage);
+            const uint32_t kb = ring_k + (e % kStages) * (Cfg::kStage >> 4);
 #pragma unroll
             for (int part = 0; part < kParts; ++part) {
-              const uint32_t qb = ptx::smem_addr(sq + (x * kParts + part) * Cfg::kQTile);
+              const uint32_t qb = q_k + (x * kParts + part) * (Cfg::kQTile >> 4);
 #pragma unroll
-              for (int k = 0; k < D / 16; ++k) {
-                const uint32_t h = k / 4, o = (k % 4) * 32;
-                umma::mma_f16(t_s[x], desc_k(qb + h * kHalfQ + o), desc_k(kb + h * kHalfKV + o), id_s, part || k);
-              }
+              for (int k = 0; k < D / 16; ++k)
+                mma_ss(t_s[x], qb + (k / 4) * (kHalfQ >> 4) + (k % 4) * 2, kb + (k / 4) * (kHalfKV >> 4) + (k % 4) * 2, id_s,
+                       part || k);
             }
             umma::mma_commit(s_full + x);
           };
@@ -319,7 +358,7 @@ __global__ void __launch_bounds__(512, 1) chunk_kernel(const AttnArgs a, void* w
               const uint32_t ev = (tile + j) * 2 + 1, ek = ev + 1;
               const bool last = j + 1 == it.tiles;
               ok = entry(ev);
-              const uint32_t vb = ptx::smem_addr(ring + (ev % kStages) * Cfg::kStage);
+              const uint32_t vb = ring_mn + (ev % kStages) * (Cfg::kStage >> 4);
               for (int x = 0; ok && x < blocks; ++x) {
                 ok = wait(p_ready + x, ns_done[x] & 1);
                 ++ns_done[x];
@@ -329,7 +368,7 @@ __global__ void __launch_bounds__(512, 1) chunk_kernel(const AttnArgs a, void* w
                 for (int part = 0; part < kParts; ++part)
 #pragma unroll
                   for (int k = 0; k < kPos / 16; ++k)
-                    mma_ts(t_o[x], t_s[x] + kParts * 32 * (k / 4) + part * 32 + (k % 4) * 8, desc_mn(vb + k * 2048, kHalfKV), id_o, j || part || k);
+                    mma_ts(t_o[x], t_s[x] + kParts * 32 * (k / 4) + part * 32 + (k % 4) * 8, vb + k * (2048 >> 4), id_o, part || k ? 1u : (uint32_t)(j > 0));
                 if (last) {
                   umma::mma_commit(o_full + x);
                 } else {
@@ -358,17 +397,24 @@ __global__ void __launch_bounds__(512, 1) chunk_kernel(const AttnArgs a, void* w
       }
       __syncwarp();
     }
-  } else if (warp >= 8) {
+  } else if (warp > 8) {
     // ------------------------------------------------------------------ loads
-    const int lt = tid - 256, lw = warp - 8;
+    const int lw = warp - 9, lt = tid - 9 * 32;  // lw 0, 1: K and V; 2: q
     uint32_t entry = 0, turn = 0, tiles = 0;
     bool ok = true, stop = false;  // this thread's waits ended in time; the role's threads agree to stop
     uint64_t* pend[kLag];  // barriers of the copies still in flight
     int np = 0;
+    // one arrival for the loaders' 64 threads, each of which has fenced its own copies
+    auto arrive = [&](uint64_t* bar) {
+      ptx::named_bar(1, Cfg::kLoaders);
+      if (lt == 0) ptx::mbar_arrive(bar);
+    };
     auto flush = [&]() {
       asm volatile("cp.async.wait_all;" ::: "memory");
       ptx::fence_proxy_async();
-      for (int i = 0; i < np; ++i) ptx::mbar_arrive(pend[i]);
+#pragma unroll
+      for (int i = 0; i < kLag; ++i)
+        if (i < np) arrive(pend[i]);
       np = 0;
     };
     auto landed = [&](uint64_t* bar) {  // the newest group is bar's; the one kLag before it is done
@@ -376,16 +422,24 @@ __global__ void __launch_bounds__(512, 1) chunk_kernel(const AttnArgs a, void* w
       if (np == kLag) {
         cp_async_wait<kLag>();
         ptx::fence_proxy_async();
-        ptx::mbar_arrive(pend[0]);
+        arrive(pend[0]);
 #pragma unroll
         for (int i = 0; i + 1 < kLag; ++i) pend[i] = pend[i + 1];
         pend[kLag - 1] = bar;
       } else {
-        pend[np++] = bar;
+#pragma unroll
+        for (int i = 0; i < kLag; ++i)
+          if (i == np) pend[i] = bar;
+        ++np;
       }
     };
-    constexpr int kPieces = D * 2 / 16;          // 16-byte pieces of a 16-bit row
-    constexpr int kHop = 128 / kPieces;          // rows that the 128 threads copy at once
+    // a wait that has to last announces what has landed first
+    auto wait_free = [&](uint64_t* bar, uint32_t parity) {
+      if (np && ptx::named_bar_or(1, Cfg::kLoaders, !ptx::mbar_try_wait(bar, parity))) flush();
+      return wait(bar, parity);
+    };
+    constexpr int kPieces = D * 2 / 16;                 // 16-byte pieces of a 16-bit row
+    constexpr int kHop = Cfg::kLoaders / kPieces;       // rows that the loaders copy at once
     const int pr = lt / kPieces, pc = lt % kPieces;
     // byte offset of (row, piece) in a tile whose halves are `half` bytes apart
     auto at = [](int row, int piece, int half) { return (piece >> 3) * half + row * 128 + (((piece & 7) ^ (row & 7)) << 4); };
@@ -394,88 +448,153 @@ __global__ void __launch_bounds__(512, 1) chunk_kernel(const AttnArgs a, void* w
       if (idx >= items) continue;
       const ItemRange it = item_at<kPos, Cfg::kRows>(a, map, tokens, splits, idx, lane);
       if (it.tiles == 0) continue;
-      const int* table = a.batch.table + (long long)it.seq * a.batch.table_stride;
-      flush();
-      ok = ok && wait(q_empty, (turn & 1) ^ 1);
       const int blocks = it.rows > Cfg::kBlock ? 2 : 1;
       if constexpr (!kHalves) {
-#pragma unroll 4
-        for (int r = pr; r < blocks * Cfg::kBlock; r += kHop) {
-          const int tok = r / a.group;
-          const bool live = r < it.rows;
-          const T* src = static_cast<const T*>(a.q) + (long long)(it.q0 + (live ? it.tok0 + tok : 0)) * a.q_stride +
-                         (live ? it.head * a.group + r - tok * a.group : 0) * D + pc * 8;
-          cp_async_16(ptx::smem_addr(sq + (r / Cfg::kBlock) * Cfg::kQTile + at(r % Cfg::kBlock, pc, kHalfQ)), src, live);
+        if (lw == 2) {
+          ok = __all_sync(0xffffffffu, wait(q_empty, (turn & 1) ^ 1)) != 0;
+          stop = !ok;
+          if (stop) break;
+          constexpr int kQHop = 32 / kPieces;
+          const int qr = lane / kPieces, qc = lane % kPieces;
+#pragma unroll 8
+          for (int r = qr; r < blocks * Cfg::kBlock; r += kQHop) {
+            const int tok = r / a.group;
+            const bool live = r < it.rows;
+            const T* src = static_cast<const T*>(a.q) + (long long)(it.q0 + (live ? it.tok0 + tok : 0)) * a.q_stride +
+                           (live ? it.head * a.group + r - tok * a.group : 0) * D + qc * 8;
+            cp_async_16(ptx::smem_addr(sq + (r / Cfg::kBlock) * Cfg::kQTile + at(r % Cfg::kBlock, qc, kHalfQ)), src, live);
+          }
+          asm volatile("cp.async.wait_all;" ::: "memory");
+          ptx::fence_proxy_async();
+          ptx::mbar_arrive(q_full);
         }
-        landed(q_full);
       } else {
-        // a row is 16 or 32 lanes' four values each; 2^up puts its largest in [2^13, 2^14)
-        constexpr int kLanes = D / 4, kPerWarp = 32 / kLanes;
-        const int sub = lane % kLanes, grp = lane / kLanes;
-#pragma unroll 4
-        for (int r = lw * kPerWarp + grp; r < blocks * Cfg::kBlock; r += 4 * kPerWarp) {
-          const int tok = r / a.group;
-          float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-          if (r < it.rows)
-            x = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(a.q) + (long long)(it.q0 + it.tok0 + tok) * a.q_stride +
-                                                 (it.head * a.group + r - tok * a.group) * D + sub * 4);
-          float mx = fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
+        if (lw < 2) flush();
+        ok = ok && wait(q_empty, (turn & 1) ^ 1);
+        // four lanes a row, every fourth float4 each; 2^up puts the row's largest in [2^13, 2^14)
+        constexpr int kF4 = D / 16;  // float4s of a lane
+        const int sub = lane & 3;
+#pragma unroll 1
+        for (int r0 = lw * 8; r0 < blocks * Cfg::kBlock; r0 += 24) {
+          const int r = r0 + (lane >> 2), tok = r / a.group;
+          const bool live = r < it.rows;
+          const float* src = reinterpret_cast<const float*>(a.q) + (long long)(it.q0 + (live ? it.tok0 + tok : 0)) * a.q_stride +
+                             (live ? it.head * a.group + r - tok * a.group : 0) * D + sub * 4;
+          float4 x[kF4];
+          float mx = 0.0f;
 #pragma unroll
-          for (int o = kLanes / 2; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+          for (int k = 0; k < kF4; ++k) x[k] = *reinterpret_cast<const float4*>(src + 16 * k);
+#pragma unroll
+          for (int k = 0; k < kF4; ++k) {
+            if (!live) x[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            mx = fmaxf(mx, fmaxf(fmaxf(fabsf(x[k].x), fabsf(x[k].y)), fmaxf(fabsf(x[k].z), fabsf(x[k].w))));
+          }
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
           const int ex = (int)(__float_as_uint(mx) >> 23);
           const int up = ex == 0 || ex == 255 ? 0 : min(126, 140 - ex);
           const float mul = __uint_as_float((uint32_t)(127 + up) << 23);
-          if (sub == 0) s_up[(turn & 1) * 256 + r] = (int8_t)up;
-          x.x *= mul, x.y *= mul, x.z *= mul, x.w *= mul;
-          uint2 hi, lo;
-          hi.x = pack2(x.x, x.y, __half());
-          hi.y = pack2(x.z, x.w, __half());
-          const float2 h0 = __half22float2(*reinterpret_cast<const __half2*>(&hi.x));
-          const float2 h1 = __half22float2(*reinterpret_cast<const __half2*>(&hi.y));
-          lo.x = pack2(x.x - h0.x, x.y - h0.y, __half());
-          lo.y = pack2(x.z - h1.x, x.w - h1.y, __half());
-          uint8_t* dst = sq + (r / Cfg::kBlock) * kParts * Cfg::kQTile + at(r % Cfg::kBlock, sub >> 1, kHalfQ) + (sub & 1) * 8;
-          *reinterpret_cast<uint2*>(dst) = hi;
-          *reinterpret_cast<uint2*>(dst + Cfg::kQTile) = lo;
+          if (r < blocks * Cfg::kBlock) {
+            if (sub == 0) s_up[(turn & 1) * 256 + r] = (int8_t)up;
+#pragma unroll
+            for (int k = 0; k < kF4; ++k) {
+              const float4 y = make_float4(x[k].x * mul, x[k].y * mul, x[k].z * mul, x[k].w * mul);
+              uint2 hi, lo;
+              hi.x = pack2(y.x, y.y, __half());
+              hi.y = pack2(y.z, y.w, __half());
+              const float2 h0 = __half22float2(*reinterpret_cast<const __half2*>(&hi.x));
+              const float2 h1 = __half22float2(*reinterpret_cast<const __half2*>(&hi.y));
+              lo.x = pack2(y.x - h0.x, y.y - h0.y, __half());
+              lo.y = pack2(y.z - h1.x, y.w - h1.y, __half());
+              const int f4 = 4 * k + sub;  // float4 of the row: half a piece
+              uint8_t* dst = sq + (r / Cfg::kBlock) * kParts * Cfg::kQTile + at(r % Cfg::kBlock, f4 >> 1, kHalfQ) + (f4 & 1) * 8;
+              *reinterpret_cast<uint2*>(dst) = hi;
+              *reinterpret_cast<uint2*>(dst + Cfg::kQTile) = lo;
+            }
+          }
         }
         ptx::fence_proxy_async();
         ptx::mbar_arrive(q_full);
+        if (lw == 2) {
+          stop = !__all_sync(0xffffffffu, ok);
+          if (stop) break;
+        }
       }
-      const C* kbase = static_cast<const C*>(a.k_pages) + it.head * a.pg.head_stride + pc * 8;
-      const C* vbase = static_cast<const C*>(a.v_pages) + it.head * a.pg.head_stride + pc * 8;
-      auto page_of = [&](int j) {
-        const int pos = it.first + j * kPos + lt;
-        return j < it.tiles && pos < it.len ? table[pos / a.pg.page_size] : -1;
-      };
-      int page = page_of(0);
-      for (int j = 0; j < it.tiles; ++j) {
-        const int pos = it.first + j * kPos + lt;
-        long long off = -1;
-        if (page >= 0 && page < a.pg.num_pages)
-          off = page * a.pg.page_stride + (long long)(pos % a.pg.page_size) * a.pg.slot_stride;
-        else if (pos < it.len && a.status)
-          *a.status = 5u;
-        page = page_of(j + 1);
-        const unsigned bad = __ballot_sync(0xffffffffu, off < 0);
-        stop = ptx::named_bar_or(1, 128, !ok);  // the previous tile's offsets have been read
-        if (stop) break;
-        s_off[lt] = off;
-        if (lane == 0) s_bad[((tiles + j) & 7) * 4 + lw] = bad;
-        ptx::named_bar(1, 128);
+      if (lw < 2) {
+        const int* table = a.batch.table + (long long)it.seq * a.batch.table_stride;
+        const C* kbase = static_cast<const C*>(a.k_pages) + it.head * a.pg.head_stride + pc * 8;
+        const C* vbase = static_cast<const C*>(a.v_pages) + it.head * a.pg.head_stride + pc * 8;
+        constexpr int kLook = kPos / Cfg::kLoaders;  // positions that a thread looks up
+        // a tile's boxes: lane i holds the page of box i, looked up a tile ahead
+        const int boxes = box_rows ? kPos / box_rows : 0;
+        auto box_page = [&](int j) {
+          const int pos = it.first + j * kPos + lane * box_rows;
+          return lane < boxes && j < it.tiles && pos < it.len ? table[pos / a.pg.page_size] : -1;
+        };
+        int bpage = box_page(0);
+        for (int j = 0; j < it.tiles; ++j) {
+          const int tile0 = it.first + j * kPos;
+          if (boxes && tile0 + kPos <= it.len &&
+              __all_sync(0xffffffffu, lane >= boxes || (bpage >= 0 && bpage < a.pg.num_pages))) {
+            if (np) flush();
+            ok = __all_sync(0xffffffffu, ok) != 0;
+            if (lw == 0) {
+              if (lane == 0) *reinterpret_cast<uint4*>(s_bad + ((tiles + j) & 7) * 4) = make_uint4(0, 0, 0, 0);
 #pragma unroll 1
-        for (int kv = 0; kv < 2; ++kv) {
-          const uint32_t st = entry % kStages;
-          // the copies before the last kStages - 2 have been announced, so this wait ends
-          ok = ok && wait(empty + st, ((entry / kStages) & 1) ^ 1);
-          const uint32_t dst = ptx::smem_addr(ring + st * Cfg::kStage);
-          const C* basep = kv ? vbase : kbase;
-#pragma unroll 8
-          for (int r = pr; ok && r < kPos; r += kHop) {
-            const long long o = s_off[r];
-            cp_async_16(dst + at(r, pc, kHalfKV), basep + (o < 0 ? 0 : o), o >= 0);
+              for (int kv = 0; kv < 2; ++kv, ++entry) {
+                const uint32_t st = entry % kStages;
+                ok = ok && __all_sync(0xffffffffu, wait(empty + st, ((entry / kStages) & 1) ^ 1));
+                if (!ok) continue;
+                if (lane == 0) ptx::mbar_arrive_expect_tx(full + st, Cfg::kStage);
+                __syncwarp();
+                if (lane < boxes) {
+                  const int slot = (tile0 + lane * box_rows) % a.pg.page_size;
+                  const uint32_t dst = ptx::smem_addr(ring + st * Cfg::kStage) + lane * box_rows * 128;
+#pragma unroll
+                  for (int h = 0; h < D / 64; ++h)
+                    tma_4d(dst + h * kHalfKV, kv ? &vmap : &kmap, 64 * h, slot, it.head, bpage, full + st);
+                }
+              }
+            } else {
+              entry += 2;
+            }
+            bpage = box_page(j + 1);
+            continue;
           }
-          landed(full + st);
-          ++entry;
+          bpage = box_page(j + 1);
+          stop = ptx::named_bar_or(1, Cfg::kLoaders, !ok);  // the previous tile's offsets have been read
+          if (stop) break;
+#pragma unroll
+          for (int i = 0; i < kLook; ++i) {
+            const int pos = tile0 + i * Cfg::kLoaders + lt;
+            long long off = -1;
+            if (pos < it.len) {
+              const int page = table[pos / a.pg.page_size];
+              if (page >= 0 && page < a.pg.num_pages)
+                off = page * a.pg.page_stride + (long long)(pos % a.pg.page_size) * a.pg.slot_stride;
+              else if (a.status)
+                *a.status = 5u;
+            }
+            const unsigned bad = __ballot_sync(0xffffffffu, off < 0);
+            s_off[i * Cfg::kLoaders + lt] = off;
+            if (lane == 0) s_bad[((tiles + j) & 7) * 4 + i * (Cfg::kLoaders / 32) + lw] = bad;
+          }
+          ptx::named_bar(1, Cfg::kLoaders);
+#pragma unroll 1
+          for (int kv = 0; kv < 2; ++kv) {
+            const uint32_t st = entry % kStages;
+            const bool free = wait_free(empty + st, ((entry / kStages) & 1) ^ 1);
+            ok = ok && free;
+            const uint32_t dst = ptx::smem_addr(ring + st * Cfg::kStage);
+            const C* basep = kv ? vbase : kbase;
+#pragma unroll 8
+            for (int r = pr; ok && r < kPos; r += kHop) {
+              const long long o = s_off[r];
+              cp_async_16(dst + at(r, pc, kHalfKV), basep + (o < 0 ? 0 : o), o >= 0);
+            }
+            landed(full + st);
+            ++entry;
+          }
         }
       }
       tiles += it.tiles;
@@ -514,33 +633,26 @@ __global__ void __launch_bounds__(512, 1) chunk_kernel(const AttnArgs a, void* w
           if (!ok) break;
           umma::tc_fence_after();
           if (kHalves && j == 0) c = scale2 * __uint_as_float((uint32_t)(127 - s_up[(turn & 1) * 256 + rr]) << 23);
+          float s[kPos];
+#pragma unroll
+          for (int i = 0; i < kPos / 32; ++i) tmem_ld32(ts + 32 * i, s + 32 * i);
+          umma::tmem_wait_ld();
           const int pos0 = it.first + j * kPos;
           const uint4 b4 = *reinterpret_cast<const uint4*>(s_bad + ((tiles + j) & 7) * 4);
-          const bool masked = pos0 < seen_from || pos0 + kPos - 1 > seen_to || (b4.x | b4.y | b4.z | b4.w);
-          const int hi_i = plast - pos0, lo_i = pfirst - pos0;
-          // 32 scores from column 32 i on; they are read twice, for the maximum and for the
-          // weights: 128 of them do not fit the registers of 512 threads
-          auto scores32 = [&](int i, float* s) {
-            tmem_ld32(ts + 32 * i, s);
-            umma::tmem_wait_ld();
-            if (masked) {
-              const uint32_t bw = i == 0 ? b4.x : i == 1 ? b4.y : i == 2 ? b4.z : b4.w;
+          if (pos0 < seen_from || pos0 + kPos - 1 > seen_to || (b4.x | b4.y | b4.z | b4.w)) {
+            const uint32_t bw[4] = {b4.x, b4.y, b4.z, b4.w};
+            const int hi = plast - pos0, lo = pfirst - pos0;
 #pragma unroll
-              for (int k = 0; k < 32; ++k)
-                if (32 * i + k > hi_i || 32 * i + k < lo_i || ((bw >> k) & 1)) s[k] = -INFINITY;
-            }
-          };
-          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-          for (int i = 0; i < kPos / 32; ++i) {
-            float s[32];
-            scores32(i, s);
-#pragma unroll
-            for (int k = 0; k < 32; k += 8) {
-#pragma unroll
-              for (int q = 0; q < 4; ++q) mx[q] = fmaxf(mx[q], fmaxf(s[k + q], s[k + 4 + q]));
-            }
+            for (int i = 0; i < kPos; ++i)
+              if (i > hi || i < lo || ((bw[i >> 5] >> (i & 31)) & 1)) s[i] = -INFINITY;
           }
+          float mx[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+          for (int i = 4; i + 7 < kPos; i += 8)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) mx[q] = fmaxf(mx[q], fmaxf(s[i + q], s[i + 4 + q]));
+#pragma unroll
+          for (int q = 0; q < 4; ++q) mx[q] = fmaxf(mx[q], s[kPos - 4 + q]);
           const float top_x = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c;
           const bool raise = top_x > m + kSlack || (m == -INFINITY && top_x > m);
           if (__any_sync(0xffffffffu, raise)) {
@@ -549,40 +661,38 @@ __global__ void __launch_bounds__(512, 1) chunk_kernel(const AttnArgs a, void* w
             m = mn;
             l *= f;
             if (j > 0) {
-              for (int i = 0; i < D / 32; ++i) {
-                float o[32];
-                tmem_ld32(to + 32 * i, o);
+#pragma unroll 1
+              for (int i = 0; i < D / 16; ++i) {
+                float o[16];
+                tmem_ld16(to + 16 * i, o);
                 umma::tmem_wait_ld();
 #pragma unroll
-                for (int k = 0; k < 32; ++k) o[k] *= f;
-                tmem_st32(to + 32 * i, reinterpret_cast<const uint32_t*>(o));
+                for (int k = 0; k < 16; ++k) o[k] *= f;
+                tmem_st16(to + 16 * i, reinterpret_cast<const uint32_t*>(o));
               }
             }
           }
           const float sub = (m == -INFINITY ? 0.0f : m) - kShift;
-          float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+          const float2 c2 = make_float2(c, c), sub2 = make_float2(-sub, -sub);
+          float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
           for (int b = 0; b < kPos / 64; ++b) {  // 64 scores become 32 columns of weights (and 32 of lower halves)
-            float s[64];
             uint32_t hi[32];
-            scores32(2 * b, s);
-            scores32(2 * b + 1, s + 32);
 #pragma unroll
             for (int i = 0; i < 32; ++i) {
-              const float u = exp2_approx(__fmaf_rn(s[2 * i], c, -sub));
-              const float v = exp2_approx(__fmaf_rn(s[2 * i + 1], c, -sub));
-              sum[2 * (i & 1)] += u;
-              sum[2 * (i & 1) + 1] += v;
-              hi[i] = pack2(u, v, C());
+              const float2 y = __ffma2_rn(make_float2(s[64 * b + 2 * i], s[64 * b + 2 * i + 1]), c2, sub2);
+              const float2 e = make_float2(exp2_approx(y.x), exp2_approx(y.y));
+              sum[i & 1] = __fadd2_rn(sum[i & 1], e);
+              hi[i] = pack2(e.x, e.y, C());
               if constexpr (kHalves) {
                 const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&hi[i]));
-                s[i] = __uint_as_float(pack2(u - h.x, v - h.y, __half()));
+                s[64 * b + i] = __uint_as_float(pack2(e.x - h.x, e.y - h.y, __half()));
               }
             }
             tmem_st32(ts + kParts * 32 * b, hi);
-            if constexpr (kHalves) tmem_st32(ts + 64 * b + 32, reinterpret_cast<const uint32_t*>(s));
+            if constexpr (kHalves) tmem_st32(ts + 64 * b + 32, reinterpret_cast<const uint32_t*>(s + 64 * b));
           }
-          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
           tmem_wait_st();
           umma::tc_fence_before();
           ptx::mbar_arrive(p_ready + x);
@@ -670,7 +780,7 @@ __global__ void __launch_bounds__(512, 1) chunk_kernel(const AttnArgs a, void* w
   umma::tc_fence_before();
   __syncthreads();
   if (tid == 0 && *abort_flag && a.status) *a.status = 6u;
-  if (warp == 12) {
+  if (warp == 8) {
     umma::tc_fence_after();
     umma::tmem_relinquish();
     umma::tmem_dealloc(tmem, 512);

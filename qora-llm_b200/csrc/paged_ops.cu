@@ -159,6 +159,27 @@ qora_status launch_token(const paged::AttnArgs& a, void* work, cudaStream_t s) {
   return QORA_OK;
 }
 
+// Tensor map over one layer's pages: [page][head][slot][D], boxes of box_rows slots x 64
+// elements, 128-byte swizzle. False where the map cannot describe them.
+template <typename C>
+bool encode_pages(CUtensorMap* m, const void* base, const paged::AttnArgs& a, int D, int box_rows) {
+  PFN_cuTensorMapEncodeTiled_v12000 enc = tensor_map_encoder();
+  if (!enc) return false;
+  const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)a.pg.page_size, (cuuint64_t)a.hk, (cuuint64_t)a.pg.num_pages};
+  // the stride of a dimension of one is free: any valid number does
+  const cuuint64_t row = (cuuint64_t)D * sizeof(C);
+  const cuuint64_t strides[3] = {(cuuint64_t)a.pg.slot_stride * sizeof(C), a.hk > 1 ? (cuuint64_t)a.pg.head_stride * sizeof(C) : row,
+                                 a.pg.num_pages > 1 ? (cuuint64_t)a.pg.page_stride * sizeof(C) : row};
+  for (cuuint64_t s : strides)
+    if (s >= (1ull << 40)) return false;
+  const cuuint32_t box[4] = {64, (cuuint32_t)box_rows, 1, 1};
+  const cuuint32_t ones[4] = {1, 1, 1, 1};
+  const CUtensorMapDataType type =
+      std::is_same<C, __nv_bfloat16>::value ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  return enc(m, type, 4, const_cast<void*>(base), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <typename T, typename C, int D>
 qora_status launch_chunk(const paged::AttnArgs& a, void* work, cudaStream_t s) {
   using Cfg = paged::ChunkCfg<T, C, D>;
@@ -173,7 +194,14 @@ qora_status launch_chunk(const paged::AttnArgs& a, void* work, cudaStream_t s) {
   if (most > 0x7fffffff / sms) return fail(QORA_ERR_INVALID, "%d rows of %d sequences", a.batch.rows, a.batch.seqs);
   const int splits = most >= sms ? 1 : (int)(sms / most);
   const int ctas = (int)std::min<long long>(sms, most * splits);
-  paged::chunk_kernel<T, C, D><<<ctas, Cfg::kThreads, Cfg::kSmem, s>>>(a, work, tokens, splits, (int)(most * splits));
+  // boxes of a page, or of 128 rows of one: whole swizzle groups of 8 rows
+  const int ps = a.pg.page_size;
+  int box_rows = ps % Cfg::kPos == 0 ? Cfg::kPos : Cfg::kPos % ps == 0 && ps >= 8 ? ps : 0;
+  CUtensorMap kmap{}, vmap{};
+  if (box_rows && !(encode_pages<C>(&kmap, a.k_pages, a, D, box_rows) && encode_pages<C>(&vmap, a.v_pages, a, D, box_rows)))
+    box_rows = 0;
+  paged::chunk_kernel<T, C, D><<<ctas, Cfg::kThreads, Cfg::kSmem, s>>>(a, work, tokens, splits, (int)(most * splits), box_rows, kmap,
+                                                                          vmap);
   QCUDA(cudaGetLastError());
   if (splits == 1) return QORA_OK;
   cudaLaunchConfig_t cfg = {};

@@ -27,8 +27,6 @@
 #include <thread>
 #include <vector>
 
-#include <cudaTypedefs.h>
-
 #include "../../include/qora_cuda.h"
 #include "attention.cuh"
 #include "common.cuh"
@@ -2612,20 +2610,6 @@ qora_status qora_generate_greedy_batch(qora_engine* e, qora_kv* kv, const uint32
 
 // ------------------------------------------------------------------ kernel-level entries
 }  // extern "C"
-
-// cuTensorMapEncodeTiled through the runtime's driver entry point (no libcuda link)
-static PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
-  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
-  static std::once_flag once;
-  std::call_once(once, [] {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q{};
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
-  });
-  return fn;
-}
 
 // 2-D row-major tensor map over [rows][cols] elements of `esz` bytes, boxes of
 // box_cols x box_rows elements (no swizzle; rows past the end read as zero)
