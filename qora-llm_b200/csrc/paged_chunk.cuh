@@ -2,37 +2,44 @@
 // cores (tcgen05, TMEM). The time is the two products, 4 D operations per (query head, row,
 // position).
 //
-// Item. 256 packed rows of one (sequence, kv head): tokens times the kv head's query heads
-// (row r: token r / group, head r % group), so that grouped heads share every K and V tile.
-// They are two blocks of 128 rows (X = 0, 1), each with its scores (128 columns) and its
-// numerators (D columns) in TMEM; K and V tiles of 128 positions feed both. Where there are
-// fewer items than CTAs, the positions of an item are split evenly and join_kernel adds the
-// parts in order. Items are taken from the last rows (the longest runs of positions) on, in
+// Item. Two blocks (X = 0, 1) of up to 128 packed rows of one (sequence, kv head): tokens
+// times the kv head's query heads (row r: token r / group, head r % group), so that grouped
+// heads share every K and V tile. Each block has its scores and its numerators (D columns)
+// in TMEM; K and V tiles of 128 positions (64 of an f32 cache) feed both. Where there are
+// few items, the positions of an item are split evenly and chunk_join_kernel adds the parts
+// in order. Items are taken from the last rows (the longest runs of positions) on, in
 // alternating direction, so the CTAs end together.
 //
-// Roles (384 threads, one CTA per SM: a softmax thread keeps its row's 128 scores in registers):
-//   warps 0-3, 4-7   softmax of block 0, 1: a thread owns a row, reads its 128 scores from
-//                    TMEM, writes the weights back over them as the next product's operand
+// Roles (one CTA per SM):
+//   warps 0-3, 4-7   softmax of block 0, 1: a thread owns a row, keeps its scores in
+//                    registers, writes the weights back over them in TMEM as the next
+//                    product's operand
 //   warp 8           issues the products: S_X = Q_X K^T; O_X += P_X V with P_X from TMEM
-//   warps 9, 10      load K and V into the 128-byte-swizzled tiles that the products read. A
-//                    tile whose 128 positions all exist comes by TMA, a page (or 128 rows of
-//                    one) per copy, where the page size divides 128 or is a multiple of it;
-//                    other tiles are copied by cp.async in 16-byte pieces, the page looked up
-//                    per position (slots past the end become zeros)
-//   warp 11          loads q (f32 rows: warps 9-11, which split it)
+//   warps 9, 10      16-bit caches: load K and V into the 128-byte-swizzled tiles that the
+//                    products read. A tile whose 128 positions all exist comes by TMA, a page
+//                    (or 128 rows of one) per copy, where the page size divides 128 or is a
+//                    multiple of it; other tiles are copied by cp.async in 16-byte pieces,
+//                    the page looked up per position (slots past the end become zeros)
+//   warp 11          16-bit rows: loads q by TMA, the rows packed by its box (f32 rows are
+//                    loaded and split by the softmax warps)
+//   warps 9-12, 13-16   f32 caches: load K, V, and split them
 // While one block's weights are computed the other block's products run. S_X(j + 1) is
 // issued behind O_X(j), which still reads P_X(j) from the columns it overwrites: one
 // thread's products execute in order.
 //
-// f32 rows (f16 cache): q is split into binary16 upper and lower halves (22 bits, the row
-// scaled by a power of two) and so are the weights; both halves are multiplied, which
-// doubles the products.
+// f32 operands are split into binary16 upper and lower halves (22 bits) after scaling by a
+// power of two: q by row, K and V by tile (largest value in [2^13, 2^14)). The weights are
+// split too. Upper x upper, lower x upper and upper x lower are multiplied: two products
+// instead of one for an f16 cache, three for an f32 cache. The scale of K goes into the
+// scores' scale. V's scales differ from tile to tile; the numerators count in the smallest
+// so far (the largest values) and the weights of other tiles are scaled down to it.
 //
 // The running maximum is raised only when it grows by more than 2^kSlack: then the
 // numerators in TMEM are scaled, which is rare after the first tiles. Masked scores become
-// -inf before the maximum; a row that meets a non-finite value (a weight of zero times an
-// infinite value of V, or a row whose own scores are) is computed again by one warp, one
-// position at a time (row_attend).
+// -inf before the maximum. Rows that meet a non-finite value (a weight of zero times an
+// infinite value of V, or a row whose own scores are), and rows of a cache whose tiles of V
+// differ by more than 2^12 in size, are computed again by one warp, one position at a time
+// (row_attend).
 #pragma once
 
 #include <cuda.h>
@@ -48,30 +55,38 @@ namespace paged {
 
 template <typename T, typename C, int D>
 struct ChunkCfg {
-  static constexpr bool kHalves = sizeof(T) == 4;
-  static constexpr int kParts = kHalves ? 2 : 1;
+  static constexpr bool kHalves = sizeof(T) == 4;  // f32 rows: q and the weights in two halves
+  static constexpr bool kWide = sizeof(C) == 4;    // f32 cache: K and V in two halves
+  using M = typename std::conditional<kWide, __half, C>::type;  // what the tensor cores multiply
+  static constexpr int kQParts = kHalves ? 2 : 1, kParts = kWide ? 2 : 1;
   static constexpr int kBlock = 128;            // rows of a block
-  static constexpr int kRows = 2 * kBlock;      // rows of an item
-  static constexpr int kPos = 128;              // positions of a tile
+  static constexpr int kPos = kWide ? 64 : 128;  // positions of a tile
   static constexpr int kQTile = kBlock * D * 2;
-  static constexpr int kQBytes = 2 * kParts * kQTile;  // [block][part]
-  static constexpr int kStage = kPos * D * 2;
-  static constexpr int kOther = 1024 /* offsets */ + 512 /* row scales */ + 512 /* barriers, flags */;
+  static constexpr int kQBytes = 2 * kQParts * kQTile;  // [block][part]
+  static constexpr int kTile = kPos * D * 2;            // one part of a K or V tile
+  static constexpr int kStage = kParts * kTile;
+  static constexpr int kOther = 1024 /* offsets */ + 1024 /* barriers, masks, scales */;
   static constexpr int kLimit = 227 * 1024 - 1024 - kOther;
-  static constexpr int kStages = (kLimit - kQBytes) / kStage < 6 ? (kLimit - kQBytes) / kStage : 6;
+  static constexpr int kFit = (kLimit - kQBytes) / kStage;
+  static constexpr int kStages = kFit < 6 ? kFit : 6;
   static_assert(kStages >= 3, "a K tile, a V tile and the next K tile");
   static constexpr int kLag = kStages >= 4 ? 2 : 1;  // copies in flight behind the newest: at most kStages - 2
   static constexpr int kSmem = kQBytes + kStages * kStage + kOther + 1024;
-  static constexpr int kThreads = 384;
-  static constexpr int kLoaders = 64;
+  static constexpr int kLoaders = kWide ? 128 : 64;  // threads that load (f32 cache: each of K and V)
+  static constexpr int kThreads = kWide ? 544 : 384;
 };
 constexpr int kChunkMaxCtas = 160;
 constexpr unsigned long long kWaitNs = 2000000000ull;
 
-// Workspace of split items: [item] (maximum, sum) of 256 rows, then numerators [item][256][D].
-__host__ __device__ inline float2* chunk_ml(void* p) { return static_cast<float2*>(p); }
+constexpr int kChunkMaxParts = 320;  // parts of split items in one call
+// Workspace of split items: [tile and head] (first row, tokens, kv head), [part] (maximum,
+// sum) of 256 rows, numerators [part][256][D].
+__host__ __device__ inline int4* chunk_rec(void* p) { return static_cast<int4*>(p); }
+__host__ __device__ inline float2* chunk_ml(void* p) {
+  return reinterpret_cast<float2*>(static_cast<char*>(p) + kChunkMaxParts * 16);
+}
 __host__ __device__ inline float* chunk_num(void* p) {
-  return reinterpret_cast<float*>(static_cast<char*>(p) + (size_t)kChunkMaxCtas * 256 * 8);
+  return reinterpret_cast<float*>(static_cast<char*>(p) + kChunkMaxParts * 16 + (size_t)kChunkMaxParts * 256 * 8);
 }
 
 // ---------------------------------------------------------------- instructions
@@ -121,6 +136,25 @@ QORA_DEV void tmem_st16(uint32_t taddr, const uint32_t* r) {
       "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
       : "memory");
 }
+// 16 lanes x 32 columns: v[4 n + 0, 1] lane (thread / 4), columns 8 n + 2 (thread % 4) + 0, 1;
+// v[4 n + 2, 3] eight lanes on
+QORA_DEV void tmem_ld_frag(uint32_t taddr, float (&v)[16]) {
+  uint32_t* r = reinterpret_cast<uint32_t*>(v);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+// box at (x, head, row) of q
+QORA_DEV void tma_3d(uint32_t dst, const CUtensorMap* map, int x, int head, int row, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+          dst),
+      "l"(map), "r"(x), "r"(head), "r"(row), "r"(ptx::smem_addr(bar))
+      : "memory");
+}
 QORA_DEV void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // Tiles are [rows][64 elements] halves of 128-byte rows, 16-byte pieces permuted by the row
@@ -158,11 +192,14 @@ __host__ __device__ constexpr uint32_t chunk_idesc(int n, bool b_mn) {
 
 // ---------------------------------------------------------------- items
 struct ItemRange {
-  int seq, q0, n, len, head, tok0, rows;  // sequence, its first row, new rows, positions; kv head, first token, packed rows here
-  int first;                          // first position of the first tile
-  int tiles;                          // tiles of this split
-  int slot;                           // partial slot, or -1: the item is whole
+  int seq, q0, n, len, head, tok0, toks;  // sequence, its first row, new rows, positions; kv head, first token, tokens
+  int first;                              // first position of the first tile
+  int tiles;                              // tiles of this part
+  int part;                               // partial slot, or -1: the item is whole
 };
+
+// token of packed row r (< 128) of a block: r / group
+QORA_DEV int row_token(const AttnArgs& a, int r) { return (r * a.group_inv) >> 16; }
 
 // The sequences' row tiles as a warp holds them: a lane sums a run of neighbouring sequences.
 struct ItemMap {
@@ -196,10 +233,11 @@ QORA_DEV ItemMap item_map(const AttnArgs& a, int tokens, int lane) {
   return m;
 }
 // Item idx, of m.total * hk * splits; by a whole warp.
-template <int kPos, int kRows>
+template <int kPos>
 QORA_DEV ItemRange item_at(const AttnArgs& a, const ItemMap& m, int tokens, int splits, int idx, int lane) {
-  const int split = idx % splits, head = idx / splits % a.hk;
-  const int tile = m.total - 1 - idx / splits / a.hk;  // the longest runs of positions first
+  const unsigned th = (unsigned)idx / (unsigned)splits, split = (unsigned)idx - th * splits;
+  const int back = (int)(th / (unsigned)a.hk);
+  const int tile = m.total - 1 - back;  // the longest runs of positions first
   const bool here = m.upto - m.mine <= tile && tile < m.upto;
   int s = lane * m.per, base = m.upto - m.mine;
   if (here) {
@@ -217,18 +255,17 @@ QORA_DEV ItemRange item_at(const AttnArgs& a, const ItemMap& m, int tokens, int 
   r.q0 = a.batch.q_start[s];
   r.n = a.batch.q_start[s + 1] - r.q0;
   r.len = a.batch.kv_len[s];
-  r.head = head;
+  r.head = (int)th - back * a.hk;
   r.tok0 = (tile - base) * tokens;
-  const int toks = min(tokens, r.n - r.tok0);
-  r.rows = toks * a.group;
+  r.toks = min(tokens, r.n - r.tok0);
   const int p0 = r.len - r.n + r.tok0;              // position of the first row
-  const int hi = min(r.len, p0 + toks);             // positions [lo, hi) are attended to
+  const int hi = min(r.len, p0 + r.toks);           // positions [lo, hi) are attended to
   const int lo = a.window > 0 ? max(0, p0 + 1 - a.window) : 0;
   const int t0 = lo / kPos, nt = max(0, (hi + kPos - 1) / kPos - t0);
-  const int b = (int)((long long)split * nt / splits), e = (int)((long long)(split + 1) * nt / splits);
+  const int b = (int)(split * (unsigned)nt / (unsigned)splits), e = (int)((split + 1) * (unsigned)nt / (unsigned)splits);
   r.first = (t0 + b) * kPos;
   r.tiles = e - b;
-  r.slot = splits > 1 ? idx : -1;
+  r.part = splits > 1 ? idx : -1;
   return r;
 }
 
@@ -264,37 +301,61 @@ QORA_DEV void row_attend(const AttnArgs& a, const T* q, const int* table, int he
   }
 }
 
+// Four consecutive f32 values, scaled, as binary16 upper and lower halves.
+QORA_DEV void split4(const float4& x, float mul, uint2& hi, uint2& lo) {
+  const float4 y = make_float4(x.x * mul, x.y * mul, x.z * mul, x.w * mul);
+  hi.x = pack2(y.x, y.y, __half());
+  hi.y = pack2(y.z, y.w, __half());
+  const float2 h0 = __half22float2(*reinterpret_cast<const __half2*>(&hi.x));
+  const float2 h1 = __half22float2(*reinterpret_cast<const __half2*>(&hi.y));
+  lo.x = pack2(y.x - h0.x, y.y - h0.y, __half());
+  lo.y = pack2(y.z - h1.x, y.w - h1.y, __half());
+}
+// e such that 2^e brings a largest magnitude (its bits) to [2^13, 2^14); 2^e and 2^-e are normal
+QORA_DEV int scale_up(uint32_t bits) { return min(126, 140 - (int)(bits >> 23)); }
+QORA_DEV float pow2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
+constexpr int kNoScale = 127;  // a tile of zeros
+
+// byte offset of 16-byte piece `piece` of a row in a tile whose 64-element halves are `half` bytes apart
+QORA_DEV int tile_at(int row, int piece, int half) { return (piece >> 3) * half + row * 128 + (((piece & 7) ^ (row & 7)) << 4); }
+
 template <typename T, typename C, int D>
-__global__ void __launch_bounds__(384, 1) chunk_kernel(const AttnArgs a, void* work, int tokens, int splits, int max_items, int box_rows,
-                                                       const __grid_constant__ CUtensorMap kmap,
-                                                       const __grid_constant__ CUtensorMap vmap) {
+__global__ void __launch_bounds__(ChunkCfg<T, C, D>::kThreads, 1)
+    chunk_kernel(const AttnArgs a, void* work, int splits, int max_items, int box_rows,
+                 const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
+                 const __grid_constant__ CUtensorMap vmap) {
   using Cfg = ChunkCfg<T, C, D>;
-  constexpr bool kHalves = Cfg::kHalves;
-  constexpr int kPos = Cfg::kPos, kParts = Cfg::kParts, kStages = Cfg::kStages, kLag = Cfg::kLag;
+  using M = typename Cfg::M;
+  constexpr bool kHalves = Cfg::kHalves, kWide = Cfg::kWide;
+  constexpr int kPos = Cfg::kPos, kStages = Cfg::kStages, kLag = Cfg::kLag, kLoaders = Cfg::kLoaders;
   constexpr int kHalfQ = Cfg::kBlock * 128, kHalfKV = kPos * 128;  // bytes from one 64-element half to the next
+  constexpr int kProducts = kWide ? 3 : kHalves ? 2 : 1;           // (part of the left, of the right operand)
+  constexpr int kLeft[3] = {0, 1, 0}, kRight[3] = {0, 0, 1};
   extern __shared__ uint8_t smem_raw[];
   uint8_t* const smem = smem_raw + ((1024u - (ptx::smem_addr(smem_raw) & 1023u)) & 1023u);
   uint8_t* const sq = smem;
   uint8_t* const ring = smem + Cfg::kQBytes;
-  long long* const s_off = reinterpret_cast<long long*>(ring + kStages * Cfg::kStage);  // [128]
-  int8_t* const s_up = reinterpret_cast<int8_t*>(s_off + 128);  // [2 turns][256] exponents of the row scales
-  uint64_t* const bars = reinterpret_cast<uint64_t*>(s_up + 512);
-  uint64_t *const full = bars, *const empty = bars + 8, *const q_full = bars + 16, *const q_empty = bars + 17,
-           *const s_full = bars + 18, *const p_ready = bars + 20, *const o_full = bars + 22, *const done = bars + 24;
+  long long* const s_off = reinterpret_cast<long long*>(ring + kStages * Cfg::kStage);  // [128], or [K, V][64]
+  uint64_t* const bars = reinterpret_cast<uint64_t*>(s_off + 128);
+  uint64_t *const full = bars, *const empty = bars + 8, *const q_full = bars + 16, *const s_full = bars + 18,
+           *const p_ready = bars + 20, *const o_full = bars + 22, *const q_empty = bars + 24, *const done = bars + 25;
   uint32_t* const s_bad = reinterpret_cast<uint32_t*>(bars + 26);  // [8 tiles][4] positions that there are not
-  uint32_t* const s_tmem = s_bad + 32;
-  volatile int* const abort_flag = reinterpret_cast<volatile int*>(s_bad + 33);
+  int* const s_exp = reinterpret_cast<int*>(s_bad + 32);           // [8 tiles][K, V] scales of the tiles
+  uint32_t* const s_max = reinterpret_cast<uint32_t*>(s_exp + 16);  // [K, V][4 warps]
+  uint32_t* const s_tmem = s_max + 8;
+  volatile int* const abort_flag = reinterpret_cast<volatile int*>(s_tmem + 1);
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int block_toks = Cfg::kBlock / a.group, tokens = 2 * block_toks;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (tid == 0) {
     for (int i = 0; i < kStages; ++i) {
       ptx::mbar_init(full + i, 1);
       ptx::mbar_init(empty + i, 1);
     }
-    ptx::mbar_init(q_full, kHalves ? 96 : 32);
     ptx::mbar_init(q_empty, 1);
     for (int x = 0; x < 2; ++x) {
+      ptx::mbar_init(q_full + x, kHalves ? 128 : 1);
       ptx::mbar_init(s_full + x, 1);
       ptx::mbar_init(p_ready + x, 128);
       ptx::mbar_init(o_full + x, 1);
@@ -304,109 +365,138 @@ __global__ void __launch_bounds__(384, 1) chunk_kernel(const AttnArgs a, void* w
     ptx::fence_mbar_init();
   }
   if (warp == 8) umma::tmem_alloc(s_tmem, 512);
+  const ItemMap map = item_map(a, tokens, lane);
   umma::tc_fence_before();
   __syncthreads();
   umma::tc_fence_after();
   const uint32_t tmem = *s_tmem;
-  const uint32_t t_s[2] = {tmem, tmem + 128};
-  const uint32_t t_o[2] = {tmem + 256, tmem + 256 + D};
-  const ItemMap map = item_map(a, tokens, lane);
   // more row tiles than the rows can hold: the sequences' row ranges overlap
   const bool too_many = (long long)map.total * a.hk * splits > max_items;
   if (too_many && tid == 0 && a.status) *a.status = 5u;
   const int items = too_many ? 0 : map.total * a.hk * splits;
   const int ctas = (int)gridDim.x, cta = (int)blockIdx.x;
+  if (splits > 1 && cta == 0) {  // no rows for the join in the tiles that there are not
+    for (int i = items / splits + tid; i < max_items / splits; i += Cfg::kThreads) chunk_rec(work)[i] = make_int4(0, 0, 0, 0);
+  }
   // item of turn w: alternating direction, so that long and short items pair up
   auto item_of = [&](int w) { return w * ctas + (w & 1 ? ctas - 1 - cta : cta); };
   auto wait = [&](uint64_t* bar, uint32_t parity) { return umma::wait_bar(bar, parity, kWaitNs, abort_flag); };
 
   if (warp == 8) {
-    {
-      // ---------------------------------------------------------------- products
-      uint32_t tile = 0, turn = 0, ns_done[2] = {0, 0};
-      bool ok = true;
-      const uint32_t q_k = desc_k(ptx::smem_addr(sq)), ring_k = desc_k(ptx::smem_addr(ring)),
-                     ring_mn = desc_mn(ptx::smem_addr(ring), kHalfKV);
-      constexpr uint32_t id_s = chunk_idesc<C>(kPos, false), id_o = chunk_idesc<C>(D, true);
-      for (int w = 0; ok && w * ctas < items; ++w) {
+    // -------------------------------------------------------------------- products
+    uint32_t tile = 0, q_turn[2] = {0, 0}, taken[2] = {0, 0};
+    bool ok = true;
+    const uint32_t q_k = desc_k(ptx::smem_addr(sq)), ring_k = desc_k(ptx::smem_addr(ring)),
+                   ring_mn = desc_mn(ptx::smem_addr(ring), kHalfKV);
+    constexpr uint32_t id_s = chunk_idesc<M>(kPos, false), id_o = chunk_idesc<M>(D, true);
+    for (int w = 0; ok && w * ctas < items; ++w) {
+      const int idx = item_of(w);
+      if (idx >= items) continue;
+      const ItemRange it = item_at<kPos>(a, map, tokens, splits, idx, lane);
+      if (it.tiles == 0) continue;
+      const int blocks = it.toks > block_toks ? 2 : 1;
+      if (lane == 0) {
+        // ring entries alternate K, V: entry e lies in stage e % kStages
+        auto entry = [&](uint32_t e) { return wait(full + e % kStages, (e / kStages) & 1); };
+        auto scores = [&](int x, uint32_t e) {
+          const uint32_t kb = ring_k + (e % kStages) * (Cfg::kStage >> 4), qb = q_k + x * Cfg::kQParts * (Cfg::kQTile >> 4);
+#pragma unroll
+          for (int p = 0; p < kProducts; ++p)
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k)
+              mma_ss(tmem + x * 128, qb + kLeft[p] * (Cfg::kQTile >> 4) + (k / 4) * (kHalfQ >> 4) + (k % 4) * 2,
+                     kb + kRight[p] * (Cfg::kTile >> 4) + (k / 4) * (kHalfKV >> 4) + (k % 4) * 2, id_s, p || k);
+          umma::mma_commit(s_full + x);
+        };
+        ok = entry(tile * 2);
+        for (int x = 0; ok && x < blocks; ++x) {
+          ok = wait(q_full + x, q_turn[x] & 1);
+          ++q_turn[x];
+          umma::tc_fence_after();
+          if (ok) scores(x, tile * 2);
+        }
+        if (ok) {
+          umma::mma_commit(empty + (tile * 2) % kStages);
+          for (int j = 0; ok && j < it.tiles; ++j) {
+            const uint32_t ev = (tile + j) * 2 + 1, ek = ev + 1;
+            const bool last = j + 1 == it.tiles;
+            ok = entry(ev);
+            const uint32_t vb = ring_mn + (ev % kStages) * (Cfg::kStage >> 4);
+            for (int x = 0; ok && x < blocks; ++x) {
+              ok = wait(p_ready + x, taken[x] & 1);
+              ++taken[x];
+              umma::tc_fence_after();
+              if (!ok) break;
+              // 64 weights are 32 columns, their lower halves the next 32
+#pragma unroll
+              for (int p = 0; p < kProducts; ++p)
+#pragma unroll
+                for (int k = 0; k < kPos / 16; ++k)
+                  mma_ts(tmem + 256 + x * D, tmem + x * 128 + Cfg::kQParts * 32 * (k / 4) + kLeft[p] * 32 + (k % 4) * 8,
+                         vb + kRight[p] * (Cfg::kTile >> 4) + k * (2048 >> 4), id_o, p || k ? 1u : (uint32_t)(j > 0));
+              if (last) {
+                umma::mma_commit(o_full + x);
+              } else {
+                if (x == 0) {
+                  ok = entry(ek);
+                  umma::tc_fence_after();
+                }
+                if (ok) scores(x, ek);
+              }
+            }
+            if (!ok) break;
+            umma::mma_commit(empty + ev % kStages);
+            if (!last) umma::mma_commit(empty + ek % kStages);
+          }
+          umma::mma_commit(q_empty);
+        }
+      }
+      ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+      tile += it.tiles;
+    }
+    // every product has completed before the TMEM goes
+    if (lane == 0) {
+      umma::mma_commit(done);
+      umma::wait_bar(done, 0, kWaitNs, abort_flag);
+    }
+    __syncwarp();
+  } else if (!kWide && warp == 11) {
+    // -------------------------------------------------------------------- q of 16-bit rows
+    if constexpr (!kHalves) {
+      uint32_t turn = 0;
+      for (int w = 0; w * ctas < items; ++w) {
         const int idx = item_of(w);
         if (idx >= items) continue;
-        const ItemRange it = item_at<kPos, Cfg::kRows>(a, map, tokens, splits, idx, lane);
+        const ItemRange it = item_at<kPos>(a, map, tokens, splits, idx, lane);
         if (it.tiles == 0) continue;
-        const int blocks = it.rows > Cfg::kBlock ? 2 : 1;
+        if (!__all_sync(0xffffffffu, wait(q_empty, (turn & 1) ^ 1))) break;
+        const int blocks = it.toks > block_toks ? 2 : 1;
         if (lane == 0) {
-          // ring entries alternate K, V: entry e lies in stage e % kStages
-          auto entry = [&](uint32_t e) { return wait(full + e % kStages, (e / kStages) & 1); };
-          auto scores = [&](int x, uint32_t e) {
-            const uint32_t kb = ring_k + (e % kStages) * (Cfg::kStage >> 4);
-#pragma unroll
-            for (int part = 0; part < kParts; ++part) {
-              const uint32_t qb = q_k + (x * kParts + part) * (Cfg::kQTile >> 4);
-#pragma unroll
-              for (int k = 0; k < D / 16; ++k)
-                mma_ss(t_s[x], qb + (k / 4) * (kHalfQ >> 4) + (k % 4) * 2, kb + (k / 4) * (kHalfKV >> 4) + (k % 4) * 2, id_s,
-                       part || k);
-            }
-            umma::mma_commit(s_full + x);
-          };
-          ok = wait(q_full, turn & 1) && entry(tile * 2);
-          umma::tc_fence_after();
-          if (ok) {
-            for (int x = 0; x < blocks; ++x) scores(x, tile * 2);
-            umma::mma_commit(empty + (tile * 2) % kStages);
-            for (int j = 0; ok && j < it.tiles; ++j) {
-              const uint32_t ev = (tile + j) * 2 + 1, ek = ev + 1;
-              const bool last = j + 1 == it.tiles;
-              ok = entry(ev);
-              const uint32_t vb = ring_mn + (ev % kStages) * (Cfg::kStage >> 4);
-              for (int x = 0; ok && x < blocks; ++x) {
-                ok = wait(p_ready + x, ns_done[x] & 1);
-                ++ns_done[x];
-                umma::tc_fence_after();
-                if (!ok) break;
-#pragma unroll
-                for (int part = 0; part < kParts; ++part)
-#pragma unroll
-                  for (int k = 0; k < kPos / 16; ++k)
-                    mma_ts(t_o[x], t_s[x] + kParts * 32 * (k / 4) + part * 32 + (k % 4) * 8, vb + k * (2048 >> 4), id_o, part || k ? 1u : (uint32_t)(j > 0));
-                if (last) {
-                  umma::mma_commit(o_full + x);
-                } else {
-                  if (x == 0) {
-                    ok = entry(ek);
-                    umma::tc_fence_after();
-                  }
-                  if (ok) scores(x, ek);
-                }
-              }
-              if (!ok) break;
-              umma::mma_commit(empty + ev % kStages);
-              if (!last) umma::mma_commit(empty + ek % kStages);
-            }
-            umma::mma_commit(q_empty);
+          // a box is block_toks tokens x the group's heads x 64 elements: packed rows (rows
+          // past the last token are other rows, or zeros: their results are not written)
+          for (int x = 0; x < blocks; ++x) {
+            ptx::mbar_arrive_expect_tx(q_full + x, block_toks * a.group * D * 2);
+            for (int h = 0; h < D / 64; ++h)
+              tma_3d(ptx::smem_addr(sq + x * Cfg::kQTile + h * kHalfQ), &qmap, 64 * h, it.head * a.group,
+                     it.q0 + it.tok0 + x * block_toks, q_full + x);
           }
         }
-        ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
-        tile += it.tiles;
+        __syncwarp();
         ++turn;
       }
-      // every product has completed before the TMEM goes
-      if (lane == 0) {
-        umma::mma_commit(done);
-        umma::wait_bar(done, 0, kWaitNs, abort_flag);
-      }
-      __syncwarp();
     }
   } else if (warp > 8) {
-    // ------------------------------------------------------------------ loads
-    const int lw = warp - 9, lt = tid - 9 * 32;  // lw 0, 1: K and V; 2: q
-    uint32_t entry = 0, turn = 0, tiles = 0;
-    bool ok = true, stop = false;  // this thread's waits ended in time; the role's threads agree to stop
-    uint64_t* pend[kLag];  // barriers of the copies still in flight
+    // -------------------------------------------------------------------- K and V
+    const int team = kWide ? (warp - 9) >> 2 : 0;          // f32 cache: 0 loads K, 1 loads V
+    const int lt = tid - 9 * 32 - team * 128, lw = lt >> 5;  // thread and warp of the team
+    const int bar_id = 1 + team;
+    uint32_t entry = kWide ? team : 0, tiles = 0;
+    bool ok = true, stop = false;  // this thread's waits ended in time; the team's threads agree to stop
+    uint64_t* pend[kLag];          // barriers of the copies still in flight
     int np = 0;
-    // one arrival for the loaders' 64 threads, each of which has fenced its own copies
+    // one arrival for the team's threads, each of which has fenced its own writes
     auto arrive = [&](uint64_t* bar) {
-      ptx::named_bar(1, Cfg::kLoaders);
+      ptx::named_bar(bar_id, kLoaders);
       if (lt == 0) ptx::mbar_arrive(bar);
     };
     auto flush = [&]() {
@@ -435,111 +525,33 @@ __global__ void __launch_bounds__(384, 1) chunk_kernel(const AttnArgs a, void* w
     };
     // a wait that has to last announces what has landed first
     auto wait_free = [&](uint64_t* bar, uint32_t parity) {
-      if (np && ptx::named_bar_or(1, Cfg::kLoaders, !ptx::mbar_try_wait(bar, parity))) flush();
+      if (np && ptx::named_bar_or(bar_id, kLoaders, !ptx::mbar_try_wait(bar, parity))) flush();
       return wait(bar, parity);
     };
-    constexpr int kPieces = D * 2 / 16;                 // 16-byte pieces of a 16-bit row
-    constexpr int kHop = Cfg::kLoaders / kPieces;       // rows that the loaders copy at once
-    const int pr = lt / kPieces, pc = lt % kPieces;
-    // byte offset of (row, piece) in a tile whose halves are `half` bytes apart
-    auto at = [](int row, int piece, int half) { return (piece >> 3) * half + row * 128 + (((piece & 7) ^ (row & 7)) << 4); };
     for (int w = 0; !stop && w * ctas < items; ++w) {
       const int idx = item_of(w);
       if (idx >= items) continue;
-      const ItemRange it = item_at<kPos, Cfg::kRows>(a, map, tokens, splits, idx, lane);
+      const ItemRange it = item_at<kPos>(a, map, tokens, splits, idx, lane);
       if (it.tiles == 0) continue;
-      const int blocks = it.rows > Cfg::kBlock ? 2 : 1;
-      if constexpr (!kHalves) {
-        if (lw == 2) {
-          ok = __all_sync(0xffffffffu, wait(q_empty, (turn & 1) ^ 1)) != 0;
-          stop = !ok;
-          if (stop) break;
-          constexpr int kQHop = 32 / kPieces;
-          const int qr = lane / kPieces, qc = lane % kPieces;
-#pragma unroll 8
-          for (int r = qr; r < blocks * Cfg::kBlock; r += kQHop) {
-            const int tok = r / a.group;
-            const bool live = r < it.rows;
-            const T* src = static_cast<const T*>(a.q) + (long long)(it.q0 + (live ? it.tok0 + tok : 0)) * a.q_stride +
-                           (live ? it.head * a.group + r - tok * a.group : 0) * D + qc * 8;
-            cp_async_16(ptx::smem_addr(sq + (r / Cfg::kBlock) * Cfg::kQTile + at(r % Cfg::kBlock, qc, kHalfQ)), src, live);
-          }
-          asm volatile("cp.async.wait_all;" ::: "memory");
-          ptx::fence_proxy_async();
-          ptx::mbar_arrive(q_full);
-        }
-      } else {
-        if (lw < 2) flush();
-        ok = ok && wait(q_empty, (turn & 1) ^ 1);
-        // four lanes a row, every fourth float4 each; 2^up puts the row's largest in [2^13, 2^14)
-        constexpr int kF4 = D / 16;  // float4s of a lane
-        const int sub = lane & 3;
-#pragma unroll 1
-        for (int r0 = lw * 8; r0 < blocks * Cfg::kBlock; r0 += 24) {
-          const int r = r0 + (lane >> 2), tok = r / a.group;
-          const bool live = r < it.rows;
-          const float* src = reinterpret_cast<const float*>(a.q) + (long long)(it.q0 + (live ? it.tok0 + tok : 0)) * a.q_stride +
-                             (live ? it.head * a.group + r - tok * a.group : 0) * D + sub * 4;
-          float4 x[kF4];
-          float mx = 0.0f;
-#pragma unroll
-          for (int k = 0; k < kF4; ++k) x[k] = *reinterpret_cast<const float4*>(src + 16 * k);
-#pragma unroll
-          for (int k = 0; k < kF4; ++k) {
-            if (!live) x[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            mx = fmaxf(mx, fmaxf(fmaxf(fabsf(x[k].x), fabsf(x[k].y)), fmaxf(fabsf(x[k].z), fabsf(x[k].w))));
-          }
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-          const int ex = (int)(__float_as_uint(mx) >> 23);
-          const int up = ex == 0 || ex == 255 ? 0 : min(126, 140 - ex);
-          const float mul = __uint_as_float((uint32_t)(127 + up) << 23);
-          if (r < blocks * Cfg::kBlock) {
-            if (sub == 0) s_up[(turn & 1) * 256 + r] = (int8_t)up;
-#pragma unroll
-            for (int k = 0; k < kF4; ++k) {
-              const float4 y = make_float4(x[k].x * mul, x[k].y * mul, x[k].z * mul, x[k].w * mul);
-              uint2 hi, lo;
-              hi.x = pack2(y.x, y.y, __half());
-              hi.y = pack2(y.z, y.w, __half());
-              const float2 h0 = __half22float2(*reinterpret_cast<const __half2*>(&hi.x));
-              const float2 h1 = __half22float2(*reinterpret_cast<const __half2*>(&hi.y));
-              lo.x = pack2(y.x - h0.x, y.y - h0.y, __half());
-              lo.y = pack2(y.z - h1.x, y.w - h1.y, __half());
-              const int f4 = 4 * k + sub;  // float4 of the row: half a piece
-              uint8_t* dst = sq + (r / Cfg::kBlock) * kParts * Cfg::kQTile + at(r % Cfg::kBlock, f4 >> 1, kHalfQ) + (f4 & 1) * 8;
-              *reinterpret_cast<uint2*>(dst) = hi;
-              *reinterpret_cast<uint2*>(dst + Cfg::kQTile) = lo;
-            }
-          }
-        }
-        ptx::fence_proxy_async();
-        ptx::mbar_arrive(q_full);
-        if (lw == 2) {
-          stop = !__all_sync(0xffffffffu, ok);
-          if (stop) break;
-        }
-      }
-      if (lw < 2) {
-        const int* table = a.batch.table + (long long)it.seq * a.batch.table_stride;
-        const C* kbase = static_cast<const C*>(a.k_pages) + it.head * a.pg.head_stride + pc * 8;
-        const C* vbase = static_cast<const C*>(a.v_pages) + it.head * a.pg.head_stride + pc * 8;
-        constexpr int kLook = kPos / Cfg::kLoaders;  // positions that a thread looks up
-        // a tile's boxes: lane i holds the page of box i, looked up a tile ahead
-        const int boxes = box_rows ? kPos / box_rows : 0;
-        auto box_page = [&](int j) {
-          const int pos = it.first + j * kPos + lane * box_rows;
-          return lane < boxes && j < it.tiles && pos < it.len ? table[pos / a.pg.page_size] : -1;
-        };
-        int bpage = box_page(0);
-        for (int j = 0; j < it.tiles; ++j) {
-          const int tile0 = it.first + j * kPos;
+      const int* table = a.batch.table + (long long)it.seq * a.batch.table_stride;
+      const C* base = static_cast<const C*>(team ? a.v_pages : a.k_pages) + it.head * a.pg.head_stride;
+      const C* vbase = static_cast<const C*>(a.v_pages) + it.head * a.pg.head_stride;
+      // a tile's boxes: lane i holds the page of box i, looked up a tile ahead
+      const int boxes = box_rows ? kPos / box_rows : 0;
+      auto box_page = [&](int j) {
+        const int pos = it.first + j * kPos + lane * box_rows;
+        return lane < boxes && j < it.tiles && pos < it.len ? table[pos / a.pg.page_size] : -1;
+      };
+      int bpage = box_page(0);
+      for (int j = 0; j < it.tiles; ++j) {
+        const int tile0 = it.first + j * kPos, ring8 = (tiles + j) & 7;
+        if constexpr (!kWide) {
           if (boxes && tile0 + kPos <= it.len &&
               __all_sync(0xffffffffu, lane >= boxes || (bpage >= 0 && bpage < a.pg.num_pages))) {
             if (np) flush();
             ok = __all_sync(0xffffffffu, ok) != 0;
             if (lw == 0) {
-              if (lane == 0) *reinterpret_cast<uint4*>(s_bad + ((tiles + j) & 7) * 4) = make_uint4(0, 0, 0, 0);
+              if (lane == 0) *reinterpret_cast<uint4*>(s_bad + ring8 * 4) = make_uint4(0, 0, 0, 0);
 #pragma unroll 1
               for (int kv = 0; kv < 2; ++kv, ++entry) {
                 const uint32_t st = entry % kStages;
@@ -562,84 +574,196 @@ __global__ void __launch_bounds__(384, 1) chunk_kernel(const AttnArgs a, void* w
             continue;
           }
           bpage = box_page(j + 1);
-          stop = ptx::named_bar_or(1, Cfg::kLoaders, !ok);  // the previous tile's offsets have been read
-          if (stop) break;
-#pragma unroll
-          for (int i = 0; i < kLook; ++i) {
-            const int pos = tile0 + i * Cfg::kLoaders + lt;
-            long long off = -1;
-            if (pos < it.len) {
-              const int page = table[pos / a.pg.page_size];
-              if (page >= 0 && page < a.pg.num_pages)
-                off = page * a.pg.page_stride + (long long)(pos % a.pg.page_size) * a.pg.slot_stride;
-              else if (a.status)
-                *a.status = 5u;
-            }
-            const unsigned bad = __ballot_sync(0xffffffffu, off < 0);
-            s_off[i * Cfg::kLoaders + lt] = off;
-            if (lane == 0) s_bad[((tiles + j) & 7) * 4 + i * (Cfg::kLoaders / 32) + lw] = bad;
+        }
+        stop = ptx::named_bar_or(bar_id, kLoaders, !ok);  // the previous tile's offsets have been read
+        if (stop) break;
+        for (int i = lt; i < kPos; i += kLoaders) {
+          const int pos = tile0 + i;
+          long long off = -1;
+          if (pos < it.len) {
+            const int page = table[pos / a.pg.page_size];
+            if (page >= 0 && page < a.pg.num_pages)
+              off = page * a.pg.page_stride + (long long)(pos % a.pg.page_size) * a.pg.slot_stride;
+            else if (a.status)
+              *a.status = 5u;
           }
-          ptx::named_bar(1, Cfg::kLoaders);
+          const unsigned bad = __ballot_sync(0xffffffffu, off < 0);
+          s_off[team * kPos + i] = off;
+          if (lane == 0 && team == 0) s_bad[ring8 * 4 + (i >> 5)] = bad;
+        }
+        if (kWide && team == 0 && lt == 127) s_bad[ring8 * 4 + 2] = s_bad[ring8 * 4 + 3] = 0u;
+        ptx::named_bar(bar_id, kLoaders);
+        if constexpr (!kWide) {
+          constexpr int kPieces = D * 2 / 16;      // 16-byte pieces of a row
+          constexpr int kHop = kLoaders / kPieces;  // rows that the team copies at once
+          const int pr = lt / kPieces, pc = lt % kPieces;
 #pragma unroll 1
-          for (int kv = 0; kv < 2; ++kv) {
+          for (int kv = 0; kv < 2; ++kv, ++entry) {
             const uint32_t st = entry % kStages;
             const bool free = wait_free(empty + st, ((entry / kStages) & 1) ^ 1);
             ok = ok && free;
             const uint32_t dst = ptx::smem_addr(ring + st * Cfg::kStage);
-            const C* basep = kv ? vbase : kbase;
+            const C* basep = (kv ? vbase : base) + pc * 8;
 #pragma unroll 8
             for (int r = pr; ok && r < kPos; r += kHop) {
               const long long o = s_off[r];
-              cp_async_16(dst + at(r, pc, kHalfKV), basep + (o < 0 ? 0 : o), o >= 0);
+              cp_async_16(dst + tile_at(r, pc, kHalfKV), basep + (o < 0 ? 0 : o), o >= 0);
             }
             landed(full + st);
-            ++entry;
           }
+        } else {
+          constexpr int kF4 = D / 4;            // float4s of a row
+          constexpr int kHop = kLoaders / kF4;  // rows at once
+          constexpr int kN = kPos / kHop;
+          const int f4 = lt % kF4, pr = lt / kF4;
+          float4 x[kN];
+          uint32_t mx = 0;
+#pragma unroll
+          for (int i = 0; i < kN; ++i) {
+            const long long o = s_off[team * kPos + pr + i * kHop];
+            x[i] = o >= 0 ? *reinterpret_cast<const float4*>(base + o + 4 * f4) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          }
+          auto finite_bits = [](float v) {
+            const uint32_t b = __float_as_uint(v) & 0x7FFFFFFFu;
+            return b < 0x7F800000u ? b : 0u;
+          };
+#pragma unroll
+          for (int i = 0; i < kN; ++i)
+            mx = max(max(mx, max(finite_bits(x[i].x), finite_bits(x[i].y))), max(finite_bits(x[i].z), finite_bits(x[i].w)));
+          mx = __reduce_max_sync(0xffffffffu, mx);
+          if (lane == 0) s_max[team * 4 + lw] = mx;
+          const uint32_t st = entry % kStages;
+          const bool free = wait(empty + st, ((entry / kStages) & 1) ^ 1);
+          ok = ok && free;
+          ptx::named_bar(bar_id, kLoaders);
+          const uint4 m4 = *reinterpret_cast<const uint4*>(s_max + team * 4);
+          mx = max(max(m4.x, m4.y), max(m4.z, m4.w));
+          const int up = mx ? scale_up(mx) : kNoScale;
+          const float mul = mx ? pow2(up) : 1.0f;
+          if (lt == 0) s_exp[ring8 * 2 + team] = up;
+          uint8_t* dst = ring + st * Cfg::kStage;
+          if (ok) {
+#pragma unroll
+            for (int i = 0; i < kN; ++i) {
+              uint2 hi, lo;
+              split4(x[i], mul, hi, lo);
+              const int o = tile_at(pr + i * kHop, f4 >> 1, kHalfKV) + (f4 & 1) * 8;
+              *reinterpret_cast<uint2*>(dst + o) = hi;
+              *reinterpret_cast<uint2*>(dst + Cfg::kTile + o) = lo;
+            }
+          }
+          ptx::fence_proxy_async();
+          arrive(full + st);
+          entry += 2;
         }
       }
       tiles += it.tiles;
-      ++turn;
     }
     flush();
   } else {
-    // ------------------------------------------------------------------ softmax
-    const int x = warp >> 2, r = (warp & 3) * 32 + lane, rr = x * Cfg::kBlock + r;
-    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t ts = t_s[x] + lanes, to = t_o[x] + lanes;
+    // -------------------------------------------------------------------- softmax
+    const int x = warp >> 2, r0 = (warp & 3) * 32, r = r0 + lane;
+    const uint32_t ts = tmem + x * 128 + ((uint32_t)r0 << 16), to = tmem + 256 + x * D + ((uint32_t)r0 << 16);
     const float scale2 = a.scale * kLog2e;
-    uint32_t seen = 0, o_turn = 0, tiles = 0, turn = 0;
+    const int rtok = row_token(a, r);  // token of the thread's row within the block
+    uint32_t seen = 0, o_turn = 0, tiles = 0;
     bool ok = true;  // the same for the whole warp
     auto wait_all = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; };
     for (int w = 0; ok && w * ctas < items; ++w) {
       const int idx = item_of(w);
       if (idx >= items) continue;
-      const ItemRange it = item_at<kPos, Cfg::kRows>(a, map, tokens, splits, idx, lane);
-      const int block_rows = it.rows - x * Cfg::kBlock;  // of this block, if positive
-      const bool live = r < block_rows;
-      const int tok = rr / a.group, p0 = it.len - it.n + it.tok0;
-      const int plast = live ? p0 + tok : -1;
+      const ItemRange it = item_at<kPos>(a, map, tokens, splits, idx, lane);
+      const int toks = min(block_toks, it.toks - x * block_toks);  // of this block, if positive
+      const bool live = rtok < toks;
+      const int p0 = it.len - it.n + it.tok0 + x * block_toks;  // position of the block's first token
+      const int plast = live ? p0 + rtok : -1;
       const int pfirst = a.window > 0 ? max(0, plast + 1 - a.window) : 0;
-      // every row of the block sees the positions from seen_from to seen_to
-      const int seen_to = p0 + x * Cfg::kBlock / a.group;
-      const int top = p0 + (min(it.rows, (x + 1) * Cfg::kBlock) - 1) / a.group;
-      const int seen_from = a.window > 0 ? max(0, top + 1 - a.window) : 0;
-      const bool busy = block_rows > 0 && it.tiles > 0;
+      // every row of the block sees the positions from seen_from to p0
+      const int seen_from = a.window > 0 ? max(0, p0 + toks - a.window) : 0;
+      const bool busy = toks > 0 && it.tiles > 0;
+      const long long row0 = it.q0 + it.tok0 + x * block_toks;  // the block's first row
+      if (it.part >= 0 && idx % splits == 0 && tid == 0)
+        chunk_rec(work)[idx / splits] = make_int4((int)row0, it.toks, it.head, 0);
+      float c = scale2;
+      if constexpr (kHalves) {
+        // the warp's rows of q, eight at a time: four lanes a row, every fourth float4 each.
+        // The previous item's products have completed (o_full)
+        if (busy) {
+          constexpr int kF4 = D / 16;
+          const int sub = lane & 3;
+          int ups[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int rr = r0 + 8 * i + (lane >> 2), tok = row_token(a, rr);
+            const bool there = tok < toks;
+            const float* src = reinterpret_cast<const float*>(a.q) + (there ? (row0 + tok) * a.q_stride + (it.head * a.group + rr - tok * a.group) * D : 0) + sub * 4;
+            float4 y[kF4];
+            uint32_t mx = 0;
+#pragma unroll
+            for (int k = 0; k < kF4; ++k) y[k] = *reinterpret_cast<const float4*>(src + 16 * k);
+#pragma unroll
+            for (int k = 0; k < kF4; ++k) {
+              if (!there) y[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+              mx = max(max(mx, max(__float_as_uint(y[k].x) << 1, __float_as_uint(y[k].y) << 1)),
+                       max(__float_as_uint(y[k].z) << 1, __float_as_uint(y[k].w) << 1));
+            }
+            mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+            mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 2)) >> 1;
+            ups[i] = mx == 0 || mx >= 0x7F800000u ? 0 : scale_up(mx);
+            const float mul = pow2(ups[i]);
+#pragma unroll
+            for (int k = 0; k < kF4; ++k) {
+              uint2 hi, lo;
+              split4(y[k], mul, hi, lo);
+              const int f4 = 4 * k + sub;  // float4 of the row: half a piece
+              uint8_t* dst = sq + x * 2 * Cfg::kQTile + tile_at(rr, f4 >> 1, kHalfQ) + (f4 & 1) * 8;
+              *reinterpret_cast<uint2*>(dst) = hi;
+              *reinterpret_cast<uint2*>(dst + Cfg::kQTile) = lo;
+            }
+          }
+          ptx::fence_proxy_async();
+          ptx::mbar_arrive(q_full + x);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int up = __shfl_sync(0xffffffffu, ups[i], (lane & 7) * 4);
+            if ((lane >> 3) == i) c = scale2 * pow2(-up);
+          }
+        }
+      }
       float m = -INFINITY, l = 0.0f;
+      int e_ref = kNoScale;  // f32 cache: the numerators count in 2^-e_ref
+      bool wild = false;
       if (busy) {
-        float c = scale2;
         for (int j = 0; j < it.tiles; ++j) {
           ok = wait_all(s_full + x, seen & 1);
           ++seen;
           if (!ok) break;
           umma::tc_fence_after();
-          if (kHalves && j == 0) c = scale2 * __uint_as_float((uint32_t)(127 - s_up[(turn & 1) * 256 + rr]) << 23);
           float s[kPos];
 #pragma unroll
           for (int i = 0; i < kPos / 32; ++i) tmem_ld32(ts + 32 * i, s + 32 * i);
-          umma::tmem_wait_ld();
+          const int ring8 = (tiles + j) & 7;
           const int pos0 = it.first + j * kPos;
-          const uint4 b4 = *reinterpret_cast<const uint4*>(s_bad + ((tiles + j) & 7) * 4);
-          if (pos0 < seen_from || pos0 + kPos - 1 > seen_to || (b4.x | b4.y | b4.z | b4.w)) {
+          const uint4 b4 = *reinterpret_cast<const uint4*>(s_bad + ring8 * 4);
+          float ct = c, lift = 0.0f, o_scale = 1.0f, l_scale = 1.0f;
+          if constexpr (kWide) {
+            const uint32_t ev = (tiles + j) * 2 + 1;  // V's scale: its tile stays until this block's weights are used
+            ok = wait_all(full + ev % kStages, (ev / kStages) & 1);
+            if (!ok) break;
+            const int ek = s_exp[ring8 * 2], eV = s_exp[ring8 * 2 + 1];
+            if (ek != kNoScale) ct = c * pow2(-ek);
+            if (eV != kNoScale) {
+              if (eV < e_ref) {
+                if (e_ref != kNoScale) o_scale = pow2(max(-126, eV - e_ref));
+                e_ref = eV;
+              }
+              wild |= eV - e_ref > 12;
+              lift = (float)(e_ref - eV);
+              l_scale = pow2(min(126, eV - e_ref));
+            }
+          }
+          umma::tmem_wait_ld();
+          if (pos0 < seen_from || pos0 + kPos - 1 > p0 || (b4.x | b4.y | b4.z | b4.w)) {
             const uint32_t bw[4] = {b4.x, b4.y, b4.z, b4.w};
             const int hi = plast - pos0, lo = pfirst - pos0;
 #pragma unroll
@@ -653,13 +777,14 @@ __global__ void __launch_bounds__(384, 1) chunk_kernel(const AttnArgs a, void* w
             for (int q = 0; q < 4; ++q) mx[q] = fmaxf(mx[q], fmaxf(s[i + q], s[i + 4 + q]));
 #pragma unroll
           for (int q = 0; q < 4; ++q) mx[q] = fmaxf(mx[q], s[kPos - 4 + q]);
-          const float top_x = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c;
+          const float top_x = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * ct;
           const bool raise = top_x > m + kSlack || (m == -INFINITY && top_x > m);
-          if (__any_sync(0xffffffffu, raise)) {
-            const float mn = fmaxf(m, top_x);
+          if (__any_sync(0xffffffffu, raise) || (kWide && o_scale != 1.0f)) {
+            const float mn = raise ? fmaxf(m, top_x) : m;
             const float f = mn == -INFINITY ? 1.0f : exp2_approx(m - mn);
             m = mn;
             l *= f;
+            const float fo = f * o_scale;
             if (j > 0) {
 #pragma unroll 1
               for (int i = 0; i < D / 16; ++i) {
@@ -667,13 +792,13 @@ __global__ void __launch_bounds__(384, 1) chunk_kernel(const AttnArgs a, void* w
                 tmem_ld16(to + 16 * i, o);
                 umma::tmem_wait_ld();
 #pragma unroll
-                for (int k = 0; k < 16; ++k) o[k] *= f;
+                for (int k = 0; k < 16; ++k) o[k] *= fo;
                 tmem_st16(to + 16 * i, reinterpret_cast<const uint32_t*>(o));
               }
             }
           }
-          const float sub = (m == -INFINITY ? 0.0f : m) - kShift;
-          const float2 c2 = make_float2(c, c), sub2 = make_float2(-sub, -sub);
+          const float sub = (m == -INFINITY ? 0.0f : m) - kShift - lift;
+          const float2 c2 = make_float2(ct, ct), sub2 = make_float2(-sub, -sub);
           float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
           for (int b = 0; b < kPos / 64; ++b) {  // 64 scores become 32 columns of weights (and 32 of lower halves)
@@ -683,16 +808,17 @@ __global__ void __launch_bounds__(384, 1) chunk_kernel(const AttnArgs a, void* w
               const float2 y = __ffma2_rn(make_float2(s[64 * b + 2 * i], s[64 * b + 2 * i + 1]), c2, sub2);
               const float2 e = make_float2(exp2_approx(y.x), exp2_approx(y.y));
               sum[i & 1] = __fadd2_rn(sum[i & 1], e);
-              hi[i] = pack2(e.x, e.y, C());
+              hi[i] = pack2(e.x, e.y, M());
               if constexpr (kHalves) {
                 const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&hi[i]));
                 s[64 * b + i] = __uint_as_float(pack2(e.x - h.x, e.y - h.y, __half()));
               }
             }
-            tmem_st32(ts + kParts * 32 * b, hi);
+            tmem_st32(ts + Cfg::kQParts * 32 * b, hi);
             if constexpr (kHalves) tmem_st32(ts + 64 * b + 32, reinterpret_cast<const uint32_t*>(s + 64 * b));
           }
-          l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+          const float add = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+          l = kWide ? __fmaf_rn(add, l_scale, l) : l + add;
           tmem_wait_st();
           umma::tc_fence_before();
           ptx::mbar_arrive(p_ready + x);
@@ -705,74 +831,109 @@ __global__ void __launch_bounds__(384, 1) chunk_kernel(const AttnArgs a, void* w
       }
       if (!ok) break;
       tiles += it.tiles;
-      turn += it.tiles > 0;
-      if (block_rows <= 0) continue;
-      // ---- the rows' results
-      const int row = it.q0 + it.tok0 + tok, h = it.head * a.group + rr - tok * a.group;
-      bool again = false;
-      const float inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
-      T* out = static_cast<T*>(a.out) + (long long)row * a.out_stride + h * D;
-      float* num = it.slot < 0 ? nullptr : chunk_num(work) + ((size_t)it.slot * Cfg::kRows + rr) * D;
-      for (int i = 0; i < D / 32; ++i) {
-        float o[32];
-        if (busy) {
-          tmem_ld32(to + 32 * i, o);
-          umma::tmem_wait_ld();
-        } else {
-#pragma unroll
-          for (int k = 0; k < 32; ++k) o[k] = 0.0f;
-        }
-        float z = 0.0f;
-#pragma unroll
-        for (int k = 0; k < 32; ++k) z = __fmaf_rn(o[k], 0.0f, z);
-        again |= z != 0.0f;  // 0, or NaN where a numerator is not finite
-        if (live) {
-          if (it.slot < 0) {
-#pragma unroll
-            for (int k = 0; k < 32; k += 8) {
-              float y[8];
-#pragma unroll
-              for (int q = 0; q < 8; ++q) y[q] = o[k + q] * inv;
-              store_elems(out + 32 * i + k, y);
-            }
+      if (toks <= 0) continue;
+      // ---- the rows' results: 16 rows at a time, so that four threads write 32 bytes of a row
+      const float back = kWide && e_ref != kNoScale ? pow2(-e_ref) : 1.0f;
+      const float mul = it.part >= 0 ? 1.0f : l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
+      const unsigned live_rows = __ballot_sync(0xffffffffu, live);
+      unsigned redo = __ballot_sync(0xffffffffu, live && (wild || !(l * 0.0f == 0.0f)));
+#pragma unroll 1
+      for (int h = 0; h < 2; ++h) {
+        const int ra = 16 * h + (lane >> 2), t = lane & 3;  // this thread's rows: ra and ra + 8 of the warp's
+        const float mula = __shfl_sync(0xffffffffu, mul, ra), mulb = __shfl_sync(0xffffffffu, mul, ra + 8);
+        const bool la = (live_rows >> ra) & 1, lb = (live_rows >> (ra + 8)) & 1;
+        auto out_row = [&](int rr) {  // output of packed row rr of the block
+          const int tok = row_token(a, rr);
+          return static_cast<T*>(a.out) + (row0 + tok) * a.out_stride + (it.head * a.group + rr - tok * a.group) * D;
+        };
+        T* const oa = out_row(r0 + ra);
+        T* const ob = out_row(r0 + ra + 8);
+        float* const na = it.part < 0 ? nullptr : chunk_num(work) + ((size_t)it.part * 256 + x * 128 + r0 + ra) * D;
+        float za = 0.0f, zb = 0.0f;  // 0, or NaN where a numerator is not finite
+#pragma unroll 1
+        for (int cb = 0; cb < D / 32; ++cb) {
+          float v[16];
+          if (busy) {
+            tmem_ld_frag(to + ((uint32_t)(16 * h) << 16) + 32 * cb, v);
+            umma::tmem_wait_ld();
           } else {
 #pragma unroll
-            for (int k = 0; k < 32; k += 4) *reinterpret_cast<float4*>(num + 32 * i + k) = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+            for (int k = 0; k < 16; ++k) v[k] = 0.0f;
+          }
+#pragma unroll
+          for (int n = 0; n < 4; ++n) {
+            za = __fmaf_rn(v[4 * n], 0.0f, __fmaf_rn(v[4 * n + 1], 0.0f, za));
+            zb = __fmaf_rn(v[4 * n + 2], 0.0f, __fmaf_rn(v[4 * n + 3], 0.0f, zb));
+            v[4 * n] *= mula;
+            v[4 * n + 1] *= mula;
+            v[4 * n + 2] *= mulb;
+            v[4 * n + 3] *= mulb;
+            if constexpr (kWide) {  // apart from the quotient: their product may leave the normal range
+#pragma unroll
+              for (int k = 0; k < 4; ++k) v[4 * n + k] *= back;
+            }
+          }
+          if (it.part >= 0 || kHalves) {
+            float* const pa = it.part >= 0 ? na : reinterpret_cast<float*>(oa);
+            float* const pb = it.part >= 0 ? na + 8 * D : reinterpret_cast<float*>(ob);
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+              const int d = 32 * cb + 8 * n + 2 * t;
+              if (la) *reinterpret_cast<float2*>(pa + d) = make_float2(v[4 * n], v[4 * n + 1]);
+              if (lb) *reinterpret_cast<float2*>(pb + d) = make_float2(v[4 * n + 2], v[4 * n + 3]);
+            }
+          } else {
+            // neighbours trade, so that a thread has four consecutive elements of one n8 group
+#pragma unroll
+            for (int n = 0; n < 4; n += 2) {
+#pragma unroll
+              for (int q = 0; q < 2; ++q) {
+                const uint32_t w0 = pack2(v[4 * n + 2 * q], v[4 * n + 2 * q + 1], M());
+                const uint32_t w1 = pack2(v[4 * n + 4 + 2 * q], v[4 * n + 5 + 2 * q], M());
+                const uint32_t got = __shfl_xor_sync(0xffffffffu, t & 1 ? w0 : w1, 1);
+                const int d = 32 * cb + 8 * (n + (t & 1)) + 4 * (t >> 1);
+                if (q ? lb : la) *reinterpret_cast<uint2*>((q ? ob : oa) + d) = t & 1 ? make_uint2(got, w1) : make_uint2(w0, got);
+              }
+            }
           }
         }
+        const unsigned fa = __ballot_sync(0xffffffffu, za != 0.0f), fb = __ballot_sync(0xffffffffu, zb != 0.0f);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          if ((fa >> (4 * q)) & 15u) redo |= 1u << (16 * h + q);
+          if ((fb >> (4 * q)) & 15u) redo |= 1u << (16 * h + 8 + q);
+        }
       }
-      again |= !(l * 0.0f == 0.0f);
-      // rows with non-finite numerators, one after the other by the whole warp
-      unsigned redo = __ballot_sync(0xffffffffu, live && again);
+      // rows to compute again, one after the other by the whole warp
+      redo &= live_rows;
       if (redo) {
         const int* table = a.batch.table + (long long)it.seq * a.batch.table_stride;
         for (; redo; redo &= redo - 1) {
-          const int src = __ffs(redo) - 1;
-          const int r2 = rr - lane + src, tok2 = r2 / a.group;
+          const int src = __ffs(redo) - 1, rr = r0 + src, tok = row_token(a, rr);
           const int last2 = __shfl_sync(0xffffffffu, plast, src), first2 = __shfl_sync(0xffffffffu, pfirst, src);
-          const long long row2 = it.q0 + it.tok0 + tok2;
-          const int h2 = it.head * a.group + r2 - tok2 * a.group;
+          const long long row = row0 + tok;
+          const int h = it.head * a.group + rr - tok * a.group;
           float o2[D / 32], m2, l2;
-          row_attend<T, C, D>(a, static_cast<const T*>(a.q) + row2 * a.q_stride + h2 * D, table, it.head, max(first2, it.first),
+          row_attend<T, C, D>(a, static_cast<const T*>(a.q) + row * a.q_stride + h * D, table, it.head, max(first2, it.first),
                               min(last2, it.first + it.tiles * kPos - 1), scale2, o2, m2, l2);
           if (lane == src) {
             m = m2;
             l = l2;
           }
-          const float inv2 = l2 == 0.0f ? 0.0f : __fdiv_rn(1.0f, l2);
+          const float inv = l2 == 0.0f ? 0.0f : __fdiv_rn(1.0f, l2);
           for (int i = 0; i < D / 32; ++i) {
-            if (it.slot < 0)
-              static_cast<T*>(a.out)[row2 * a.out_stride + h2 * D + lane + 32 * i] = from_f32(__fmul_rn(o2[i], inv2), T());
+            if (it.part < 0)
+              static_cast<T*>(a.out)[row * a.out_stride + h * D + lane + 32 * i] = from_f32(__fmul_rn(o2[i], inv), T());
             else
-              chunk_num(work)[((size_t)it.slot * Cfg::kRows + r2) * D + lane + 32 * i] = o2[i];
+              chunk_num(work)[((size_t)it.part * 256 + x * 128 + rr) * D + lane + 32 * i] = o2[i];
           }
         }
       }
       if (live) {
-        if (it.slot >= 0)
-          chunk_ml(work)[(size_t)it.slot * Cfg::kRows + rr] = make_float2(m, l);
+        if (it.part >= 0)
+          chunk_ml(work)[(size_t)it.part * 256 + x * 128 + r] = make_float2(m, l);
         else if (a.lse)
-          a.lse[(long long)row * a.hq + h] = l == 0.0f ? -INFINITY : (m - kShift + log2f(l)) * kLn2;
+          a.lse[(row0 + rtok) * a.hq + it.head * a.group + r - rtok * a.group] = l == 0.0f ? -INFINITY : (m - kShift + log2f(l)) * kLn2;
       }
     }
   }
@@ -787,36 +948,51 @@ __global__ void __launch_bounds__(384, 1) chunk_kernel(const AttnArgs a, void* w
   }
 }
 
-// Split items: block (tile and head, group of 8 rows) adds an item's parts in order, a warp a row.
+// Split items: a warp adds the parts of a row in order; block (tile and head, group of 8 rows).
 template <typename T, int D>
-__global__ void __launch_bounds__(256) chunk_join_kernel(const AttnArgs a, void* work, int tokens, int splits) {
-  constexpr int kRows = 256, E = D / 32;
+__global__ void __launch_bounds__(256) chunk_join_kernel(const AttnArgs a, void* work, int splits) {
+  constexpr int E = D / 32, kAhead = 8;
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int lane = threadIdx.x & 31, r = blockIdx.y * 8 + (threadIdx.x >> 5);
-  const ItemMap map = item_map(a, tokens, lane);
-  const int idx = blockIdx.x * splits;
-  if ((long long)map.total * a.hk > (long long)gridDim.x || idx >= map.total * a.hk * splits) return;
-  const ItemRange it = item_at<128, kRows>(a, map, tokens, splits, idx, lane);
-  if (r >= it.rows) return;
+  const int4 rec = chunk_rec(work)[blockIdx.x];  // (first row, tokens, kv head)
+  const int lane = threadIdx.x & 31, rr = blockIdx.y * 8 + (threadIdx.x >> 5), x = rr >> 7, r = rr & 127;
+  const int block_toks = 128 / a.group, rtok = row_token(a, r), tok = x * block_toks + rtok;
+  if (rtok >= block_toks || tok >= rec.y) return;
+  const size_t first = (size_t)blockIdx.x * splits * 256 + rr;
   float mm = -INFINITY;
-  for (int s = 0; s < splits; ++s) mm = fmaxf(mm, chunk_ml(work)[(size_t)(idx + s) * kRows + r].x);
+  for (int s = lane; s < splits; s += 32) mm = fmaxf(mm, chunk_ml(work)[first + (size_t)s * 256].x);
+  mm = warp_max(mm);
   const float mu = mm == -INFINITY ? 0.0f : mm;
   float v[E], l = 0.0f;
 #pragma unroll
   for (int j = 0; j < E; ++j) v[j] = 0.0f;
-#pragma unroll 4
-  for (int s = 0; s < splits; ++s) {
-    const float2 ml = chunk_ml(work)[(size_t)(idx + s) * kRows + r];
-    const float f = exp2_approx(ml.x - mu);
-    l = __fmaf_rn(ml.y, f, l);
-    const float* p = chunk_num(work) + ((size_t)(idx + s) * kRows + r) * D + lane * E;
+#pragma unroll 1
+  for (int s0 = 0; s0 < splits; s0 += kAhead) {
+    float2 ml[kAhead];
+    float y[kAhead][E];
 #pragma unroll
-    for (int j = 0; j < E; ++j) v[j] = __fmaf_rn(p[j], f, v[j]);
+    for (int k = 0; k < kAhead; ++k) {
+      const size_t at = first + (size_t)min(s0 + k, splits - 1) * 256;
+      ml[k] = s0 + k < splits ? chunk_ml(work)[at] : make_float2(-INFINITY, 0.0f);
+      const float* p = chunk_num(work) + at * D + lane * E;
+#pragma unroll
+      for (int j = 0; j < E; j += 2) {
+        const float2 z = *reinterpret_cast<const float2*>(p + j);
+        y[k][j] = z.x;
+        y[k][j + 1] = z.y;
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      if (s0 + k >= splits) break;
+      const float f = exp2_approx(ml[k].x - mu);
+      l = __fmaf_rn(ml[k].y, f, l);
+#pragma unroll
+      for (int j = 0; j < E; ++j) v[j] = __fmaf_rn(y[k][j], f, v[j]);
+    }
   }
   const float inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
-  const int tok = r / a.group;
-  const long long row = it.q0 + it.tok0 + tok;
-  const int h = it.head * a.group + r - tok * a.group;
+  const long long row = rec.x + tok;
+  const int h = rec.z * a.group + r - rtok * a.group;
   T* out = static_cast<T*>(a.out) + row * a.out_stride + h * D + lane * E;
 #pragma unroll
   for (int j = 0; j < E; ++j) out[j] = from_f32(v[j] * inv, T());

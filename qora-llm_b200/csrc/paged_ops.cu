@@ -42,7 +42,7 @@ qora_status check_rows(const char* what, const void* p, uint64_t stride, uint32_
   if (!p) return fail(QORA_ERR_INVALID, "%s is NULL", what);
   if (((uintptr_t)p | (stride * esz)) % 16)
     return fail(QORA_ERR_INVALID, "%s: rows must start on 16-byte boundaries (stride %llu)", what, (ull)stride);
-  if (stride < (uint64_t)heads * head_dim || stride > (1ull << 40))
+  if (stride < (uint64_t)heads * head_dim || stride >= (1ull << 38))
     return fail(QORA_ERR_INVALID, "%s: row stride %llu for %u heads of %u", what, (ull)stride, heads, head_dim);
   return QORA_OK;
 }
@@ -159,25 +159,32 @@ qora_status launch_token(const paged::AttnArgs& a, void* work, cudaStream_t s) {
   return QORA_OK;
 }
 
-// Tensor map over one layer's pages: [page][head][slot][D], boxes of box_rows slots x 64
-// elements, 128-byte swizzle. False where the map cannot describe them.
+// Tensor map of 16-bit elements, 64 innermost elements per box, 128-byte swizzle. False
+// where the map cannot describe them.
 template <typename C>
-bool encode_pages(CUtensorMap* m, const void* base, const paged::AttnArgs& a, int D, int box_rows) {
+bool encode_rows(CUtensorMap* m, const void* base, int rank, const cuuint64_t* dims, const cuuint64_t* strides,
+                 const cuuint32_t* box) {
   PFN_cuTensorMapEncodeTiled_v12000 enc = tensor_map_encoder();
   if (!enc) return false;
-  const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)a.pg.page_size, (cuuint64_t)a.hk, (cuuint64_t)a.pg.num_pages};
-  // the stride of a dimension of one is free: any valid number does
-  const cuuint64_t row = (cuuint64_t)D * sizeof(C);
-  const cuuint64_t strides[3] = {(cuuint64_t)a.pg.slot_stride * sizeof(C), a.hk > 1 ? (cuuint64_t)a.pg.head_stride * sizeof(C) : row,
-                                 a.pg.num_pages > 1 ? (cuuint64_t)a.pg.page_stride * sizeof(C) : row};
-  for (cuuint64_t s : strides)
-    if (s >= (1ull << 40)) return false;
-  const cuuint32_t box[4] = {64, (cuuint32_t)box_rows, 1, 1};
+  for (int i = 0; i + 1 < rank; ++i)
+    if (strides[i] >= (1ull << 40)) return false;
   const cuuint32_t ones[4] = {1, 1, 1, 1};
   const CUtensorMapDataType type =
       std::is_same<C, __nv_bfloat16>::value ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-  return enc(m, type, 4, const_cast<void*>(base), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+  return enc(m, type, rank, const_cast<void*>(base), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// One layer's pages as [page][head][slot][D], boxes of box_rows slots.
+template <typename C>
+bool encode_pages(CUtensorMap* m, const void* base, const paged::AttnArgs& a, int D, int box_rows) {
+  const cuuint64_t row = (cuuint64_t)D * sizeof(C);
+  const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)a.pg.page_size, (cuuint64_t)a.hk, (cuuint64_t)a.pg.num_pages};
+  // the stride of a dimension of one is free: any valid number does
+  const cuuint64_t strides[3] = {(cuuint64_t)a.pg.slot_stride * sizeof(C), a.hk > 1 ? (cuuint64_t)a.pg.head_stride * sizeof(C) : row,
+                                 a.pg.num_pages > 1 ? (cuuint64_t)a.pg.page_stride * sizeof(C) : row};
+  const cuuint32_t box[4] = {64, (cuuint32_t)box_rows, 1, 1};
+  return encode_rows<C>(m, base, 4, dims, strides, box);
 }
 
 template <typename T, typename C, int D>
@@ -187,25 +194,34 @@ qora_status launch_chunk(const paged::AttnArgs& a, void* work, cudaStream_t s) {
   QCUDA(cudaGetDevice(&dev));
   QCHECK((allow_smem<&paged::chunk_kernel<T, C, D>>(dev, Cfg::kSmem)));
   const int sms = std::min(sm_count(dev), paged::kChunkMaxCtas);
-  const int tokens = Cfg::kRows / a.group;
+  const int block_toks = Cfg::kBlock / a.group, tokens = 2 * block_toks;
   // row tiles that sequences with disjoint rows can have; items of long caches are split
   // until there is one for every SM
   const long long most = ((long long)a.batch.rows + (long long)a.batch.seqs * (tokens - 1)) / tokens * a.hk;
   if (most > 0x7fffffff / sms) return fail(QORA_ERR_INVALID, "%d rows of %d sequences", a.batch.rows, a.batch.seqs);
   const int splits = most >= sms ? 1 : (int)(sms / most);
   const int ctas = (int)std::min<long long>(sms, most * splits);
-  // boxes of a page, or of 128 rows of one: whole swizzle groups of 8 rows
-  const int ps = a.pg.page_size;
-  int box_rows = ps % Cfg::kPos == 0 ? Cfg::kPos : Cfg::kPos % ps == 0 && ps >= 8 ? ps : 0;
-  CUtensorMap kmap{}, vmap{};
-  if (box_rows && !(encode_pages<C>(&kmap, a.k_pages, a, D, box_rows) && encode_pages<C>(&vmap, a.v_pages, a, D, box_rows)))
-    box_rows = 0;
-  paged::chunk_kernel<T, C, D><<<ctas, Cfg::kThreads, Cfg::kSmem, s>>>(a, work, tokens, splits, (int)(most * splits), box_rows, kmap,
-                                                                          vmap);
+  CUtensorMap qmap{}, kmap{}, vmap{};
+  int box_rows = 0;
+  if constexpr (!Cfg::kWide) {
+    // boxes of a page, or of 128 rows of one: whole swizzle groups of 8 rows
+    const int ps = a.pg.page_size;
+    box_rows = ps % Cfg::kPos == 0 ? Cfg::kPos : Cfg::kPos % ps == 0 && ps >= 8 ? ps : 0;
+    if (box_rows && !(encode_pages<C>(&kmap, a.k_pages, a, D, box_rows) && encode_pages<C>(&vmap, a.v_pages, a, D, box_rows)))
+      box_rows = 0;
+  }
+  if constexpr (!Cfg::kHalves) {
+    const cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)a.hq, (cuuint64_t)a.batch.rows};
+    const cuuint64_t strides[2] = {(cuuint64_t)D * sizeof(T), (cuuint64_t)a.q_stride * sizeof(T)};
+    const cuuint32_t box[3] = {64, (cuuint32_t)a.group, (cuuint32_t)block_toks};
+    if (!encode_rows<T>(&qmap, a.q, 3, dims, strides, box)) return fail(QORA_ERR_CUDA, "cuTensorMapEncodeTiled failed on q");
+  }
+  paged::chunk_kernel<T, C, D><<<ctas, Cfg::kThreads, Cfg::kSmem, s>>>(a, work, splits, (int)(most * splits), box_rows,
+                                                                      qmap, kmap, vmap);
   QCUDA(cudaGetLastError());
   if (splits == 1) return QORA_OK;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)most, std::min(Cfg::kRows, (int)std::min<long long>(a.max_q, tokens) * a.group + 7) / 8);
+  cfg.gridDim = dim3((unsigned)most, a.max_q > block_toks ? 32 : 16);
   cfg.blockDim = dim3(256);
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
@@ -213,18 +229,14 @@ qora_status launch_chunk(const paged::AttnArgs& a, void* work, cudaStream_t s) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  QCUDA(cudaLaunchKernelEx(&cfg, paged::chunk_join_kernel<T, D>, a, work, tokens, splits));
+  QCUDA(cudaLaunchKernelEx(&cfg, paged::chunk_join_kernel<T, D>, a, work, splits));
   return QORA_OK;
 }
 
 template <typename T, typename C, int D>
 qora_status launch_attn(const paged::AttnArgs& a, void* work, cudaStream_t s) {
   if ((long long)a.max_q * a.group <= paged::TokenCfg<T, C, D>::kRows) return launch_token<T, C, D>(a, work, s);
-  if constexpr (sizeof(C) == 2) return launch_chunk<T, C, D>(a, work, s);
-  const long long units = (long long)a.batch.rows * a.hq;
-  paged::attn_row_kernel<T, C, D><<<(unsigned)((units + 7) / 8), 256, 0, s>>>(a);
-  QCUDA(cudaGetLastError());
-  return QORA_OK;
+  return launch_chunk<T, C, D>(a, work, s);
 }
 
 template <typename T, typename C>
