@@ -74,6 +74,10 @@ struct ChunkCfg {
   static constexpr int kSmem = kQBytes + kStages * kStage + kOther + 1024;
   static constexpr int kLoaders = kWide ? 128 : 64;  // threads that load (f32 cache: each of K and V)
   static constexpr int kThreads = kWide ? 544 : 384;
+  // Scores that a softmax thread holds at once. 16-bit rows: the whole tile's (8,192 rows in
+  // 267 us; 32 at a time, read twice: 300 us, each read waits). f32 rows: 32, in small loops
+  // (512 rows over 8K positions in 85 us; the whole tile's: 92 us, registers spill).
+  static constexpr int kCols = kHalves ? 32 : kPos;
   // f32 rows: after so many tiles the numerators are added to those of the tiles before them
   // in registers, rounded to nearest. The tensor cores' own sums are cut: 16 tiles in a row
   // were off by 5.8e-6 of the result, where f32 sums are off by 1.8e-6.
@@ -337,6 +341,7 @@ __global__ void __launch_bounds__(ChunkCfg<T, C, D>::kThreads, 1)
   using Cfg = ChunkCfg<T, C, D>;
   using M = typename Cfg::M;
   constexpr bool kHalves = Cfg::kHalves, kWide = Cfg::kWide;
+  constexpr int kCols = Cfg::kCols;
   constexpr int kPos = Cfg::kPos, kStages = Cfg::kStages, kLag = Cfg::kLag, kLoaders = Cfg::kLoaders;
   constexpr int kHalfQ = Cfg::kBlock * 128, kHalfKV = kPos * 128;  // bytes from one 64-element half to the next
   constexpr int kProducts = kWide ? 3 : kHalves ? 2 : 1;           // (part of the left, of the right operand)
@@ -440,12 +445,12 @@ __global__ void __launch_bounds__(ChunkCfg<T, C, D>::kThreads, 1)
               ++taken[x];
               umma::tc_fence_after();
               if (!ok) break;
-              // 64 weights are 32 columns, their lower halves the next 32
+              // 32 weights are 16 columns, their lower halves the next 16
 #pragma unroll
               for (int p = 0; p < kProducts; ++p)
 #pragma unroll
                 for (int k = 0; k < kPos / 16; ++k)
-                  mma_ts(tmem + 256 + x * D, tmem + x * 128 + Cfg::kQParts * 32 * (k / 4) + kLeft[p] * 32 + (k % 4) * 8,
+                  mma_ts(tmem + 256 + x * D, tmem + x * 128 + Cfg::kQParts * 16 * (k / 2) + kLeft[p] * 16 + (k % 2) * 8,
                          vb + kRight[p] * (Cfg::kTile >> 4) + k * (2048 >> 4), id_o,
                          p || k ? 1u : (uint32_t)!fresh(j));
               if (last) {
@@ -790,9 +795,6 @@ __global__ void __launch_bounds__(ChunkCfg<T, C, D>::kThreads, 1)
           if (!ok) break;
           umma::tc_fence_after();
           if (kHalves && j > 0 && fresh(j)) add_up(false);
-          float s[kPos];
-#pragma unroll
-          for (int i = 0; i < kPos / 32; ++i) tmem_ld32(ts + 32 * i, s + 32 * i);
           const int ring8 = (tiles + j) & 7;
           const int pos0 = it.first + j * kPos;
           const uint4 b4 = *reinterpret_cast<const uint4*>(s_bad + ring8 * 4);
@@ -813,22 +815,39 @@ __global__ void __launch_bounds__(ChunkCfg<T, C, D>::kThreads, 1)
               l_scale = pow2(min(126, eV - e_ref));
             }
           }
-          umma::tmem_wait_ld();
-          if (pos0 < seen_from || pos0 + kPos - 1 > p0 || (b4.x | b4.y | b4.z | b4.w)) {
-            const uint32_t bw[4] = {b4.x, b4.y, b4.z, b4.w};
-            const int hi = plast - pos0, lo = pfirst - pos0;
+          const bool masked = pos0 < seen_from || pos0 + kPos - 1 > p0 || (b4.x | b4.y | b4.z | b4.w);
+          // kCols scores at a time, from TMEM for the maximum and, unless they are all, again
+          // for the weights
+          float s[kCols];
+          auto load_scores = [&](int b) {
 #pragma unroll
-            for (int i = 0; i < kPos; ++i)
-              if (i > hi || i < lo || ((bw[i >> 5] >> (i & 31)) & 1)) s[i] = -INFINITY;
+            for (int i = 0; i < kCols / 32; ++i) tmem_ld32(ts + kCols * b + 32 * i, s + 32 * i);
+            umma::tmem_wait_ld();
+            if (masked) {
+              const int hi = plast - pos0 - kCols * b, lo = pfirst - pos0 - kCols * b;
+#pragma unroll
+              for (int i = 0; i < kCols / 32; ++i) {
+                const uint32_t bw = s_bad[ring8 * 4 + (kCols / 32) * b + i];
+#pragma unroll
+                for (int k = 0; k < 32; ++k)
+                  if (32 * i + k > hi || 32 * i + k < lo || ((bw >> k) & 1)) s[32 * i + k] = -INFINITY;
+              }
+            }
+          };
+          float top_x = -INFINITY;
+#pragma unroll 1
+          for (int b = 0; b < kPos / kCols; ++b) {
+            load_scores(b);
+            float mx[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+            for (int k = 4; k + 7 < kCols; k += 8)
+#pragma unroll
+              for (int q = 0; q < 4; ++q) mx[q] = fmaxf(mx[q], fmaxf(s[k + q], s[k + 4 + q]));
+#pragma unroll
+            for (int q = 0; q < 4; ++q) mx[q] = fmaxf(mx[q], s[kCols - 4 + q]);
+            top_x = fmaxf(top_x, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
           }
-          float mx[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-          for (int i = 4; i + 7 < kPos; i += 8)
-#pragma unroll
-            for (int q = 0; q < 4; ++q) mx[q] = fmaxf(mx[q], fmaxf(s[i + q], s[i + 4 + q]));
-#pragma unroll
-          for (int q = 0; q < 4; ++q) mx[q] = fmaxf(mx[q], s[kPos - 4 + q]);
-          const float top_x = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * ct;
+          top_x *= ct;
           const bool raise = top_x > m + kSlack || (m == -INFINITY && top_x > m);
           if (__any_sync(0xffffffffu, raise) || (kWide && o_scale != 1.0f)) {
             const float mn = raise ? fmaxf(m, top_x) : m;
@@ -851,22 +870,27 @@ __global__ void __launch_bounds__(ChunkCfg<T, C, D>::kThreads, 1)
           const float sub = (m == -INFINITY ? 0.0f : m) - kShift - lift;
           const float2 c2 = make_float2(ct, ct), sub2 = make_float2(-sub, -sub);
           float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+#pragma unroll 1
+          for (int b = 0; b < kPos / kCols; ++b) {
+            if constexpr (kCols < kPos) load_scores(b);
 #pragma unroll
-          for (int b = 0; b < kPos / 64; ++b) {  // 64 scores become 32 columns of weights (and 32 of lower halves)
-            uint32_t hi[32];
+            for (int g = 0; g < kCols / 32; ++g) {  // 32 scores become 16 columns of weights (and 16 of lower halves)
+              uint32_t hi[16], lo[16];
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              const float2 y = __ffma2_rn(make_float2(s[64 * b + 2 * i], s[64 * b + 2 * i + 1]), c2, sub2);
-              const float2 e = make_float2(exp2_approx(y.x), exp2_approx(y.y));
-              sum[i & 1] = __fadd2_rn(sum[i & 1], e);
-              hi[i] = pack2(e.x, e.y, M());
-              if constexpr (kHalves) {
-                const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&hi[i]));
-                s[64 * b + i] = __uint_as_float(pack2(e.x - h.x, e.y - h.y, __half()));
+              for (int i = 0; i < 16; ++i) {
+                const float2 y = __ffma2_rn(make_float2(s[32 * g + 2 * i], s[32 * g + 2 * i + 1]), c2, sub2);
+                const float2 e = make_float2(exp2_approx(y.x), exp2_approx(y.y));
+                sum[i & 1] = __fadd2_rn(sum[i & 1], e);
+                hi[i] = pack2(e.x, e.y, M());
+                if constexpr (kHalves) {
+                  const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&hi[i]));
+                  lo[i] = pack2(e.x - h.x, e.y - h.y, __half());
+                }
               }
+              const int col = kCols * b + 32 * g;
+              tmem_st16(ts + Cfg::kQParts * (col / 2), hi);
+              if constexpr (kHalves) tmem_st16(ts + col + 16, lo);
             }
-            tmem_st32(ts + Cfg::kQParts * 32 * b, hi);
-            if constexpr (kHalves) tmem_st32(ts + 64 * b + 32, reinterpret_cast<const uint32_t*>(s + 64 * b));
           }
           const float add = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
           l = kWide ? __fmaf_rn(add, l_scale, l) : l + add;

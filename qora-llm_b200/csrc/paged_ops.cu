@@ -204,7 +204,7 @@ qora_status launch_chunk(const paged::AttnArgs& a, void* work, cudaStream_t s) {
   CUtensorMap qmap{}, kmap{}, vmap{};
   int box_rows = 0;
   if constexpr (!Cfg::kWide) {
-    // boxes of a page, or of 128 rows of one: whole swizzle groups of 8 rows
+    // boxes of a page, or of kPos rows of one: whole swizzle groups of 8 rows
     const int ps = a.pg.page_size;
     box_rows = ps % Cfg::kPos == 0 ? Cfg::kPos : Cfg::kPos % ps == 0 && ps >= 8 ? ps : 0;
     if (box_rows && !(encode_pages<C>(&kmap, a.k_pages, a, D, box_rows) && encode_pages<C>(&vmap, a.v_pages, a, D, box_rows)))
