@@ -94,24 +94,20 @@ qora_status check_batch(const int32_t* q_start, const int32_t* kv_len, const int
   return QORA_OK;
 }
 
-// Head rows a warp takes: one group where the launch is small (every load of the call in
-// flight at once), four where there are enough rows to fill the GPU either way.
-constexpr int kManyIters = 4;
-
+// Groups of head rows that a warp walks over: all of a token's, fewer while there are not
+// warps enough to fill the GPU (32 on every SM).
 template <typename T, typename C, int D, bool kAppend>
-qora_status launch_rows(const paged::RowArgs& a, cudaStream_t s) {
-  constexpr int grp = 32 / (D / 2 / paged::Elem<T>::kVec);
-  const int heads = a.hq + a.hk + a.hv;
+qora_status launch_rows(paged::RowArgs a, cudaStream_t s) {
+  constexpr int kHeads = 32 / (D / 2 / paged::Elem<T>::kVec);
+  const int groups = (a.hq + a.hk + a.hv + kHeads - 1) / kHeads;
   int dev = 0;
   QCUDA(cudaGetDevice(&dev));
-  const long long one = (long long)a.rows * ((heads + grp - 1) / grp);
-  const bool many = one > 64LL * sm_count(dev);
-  const long long units = many ? (long long)a.rows * ((heads + grp * kManyIters - 1) / (grp * kManyIters)) : one;
-  const unsigned grid = (unsigned)((units + paged::kRowWarps - 1) / paged::kRowWarps);
-  if (many)
-    paged::rows_kernel<T, C, D, kManyIters, kAppend><<<grid, 32 * paged::kRowWarps, 0, s>>>(a);
-  else
-    paged::rows_kernel<T, C, D, 1, kAppend><<<grid, 32 * paged::kRowWarps, 0, s>>>(a);
+  const long long fill = 32LL * sm_count(dev);
+  const int parts = (int)std::min<long long>(groups, (fill + a.rows - 1) / a.rows);
+  a.per_warp = (groups + parts - 1) / parts;
+  const long long units = (long long)a.rows * ((groups + a.per_warp - 1) / a.per_warp);
+  if (units > 0x7fffffff) return fail(QORA_ERR_INVALID, "%d rows of %d head rows", a.rows, a.hq + a.hk + a.hv);
+  paged::rows_kernel<T, C, D, kAppend><<<(unsigned)((units + paged::kRowWarps - 1) / paged::kRowWarps), 32 * paged::kRowWarps, 0, s>>>(a);
   QCUDA(cudaGetLastError());
   return QORA_OK;
 }

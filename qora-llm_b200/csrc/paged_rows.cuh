@@ -12,8 +12,9 @@
 // Every byte is read once and written once, so the kernel is a copy that computes on the
 // way: a lane holds one 16-byte piece of the lower half of a head row and the piece it is
 // rotated with, so the rotation needs no exchange; D/2 elements / piece = 4, 8 or 16 lanes
-// make a head row (the norm's sum is 2-4 shuffles) and a warp works on kIters groups of
-// head rows whose loads are all issued before the first is used.
+// make a head row (the norm's sum is 2-4 shuffles), 2 to 8 head rows a warp. A warp walks
+// over a token's head rows with one angle, the next ones' loads under way while it computes;
+// with few tokens their head rows are spread over more warps.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -139,6 +140,7 @@ struct RowArgs {
   int rows, hq, hk, hv;                    // hv: 0 (no append) or hk
   const float *q_gamma, *k_gamma;          // [D] or null (no norm)
   float eps;
+  int per_warp;                            // groups of head rows that a warp walks over
   const int* pos;                          // [rows] without a cache; with one, from the batch
   const float *cos_t, *sin_t;              // [rope_rows][r] or null (no rotation)
   int rope_rows, r;
@@ -151,29 +153,29 @@ struct RowArgs {
 };
 
 // T: rows, C: where k and v go (the rows' type, or the cache's). kAppend: k and v go to
-// pages. A warp handles one (row, kIters consecutive groups of head rows).
-template <typename T, typename C, int D, int kIters, bool kAppend>
-__global__ void __launch_bounds__(32 * kRowWarps) rows_kernel(const RowArgs a) {
+// pages.
+template <typename T, typename C, int D, bool kAppend>
+__global__ void __launch_bounds__(32 * kRowWarps, 4) rows_kernel(const RowArgs a) {
   constexpr int V = Elem<T>::kVec;
-  constexpr int kLanes = D / 2 / V;   // lanes of a head row
-  constexpr int kGroup_ = 32 / kLanes;  // head rows a warp holds at once
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int heads = a.hq + a.hk + a.hv;
-  const int per_row = (heads + kGroup_ * kIters - 1) / (kGroup_ * kIters);
-  const long long unit = (long long)blockIdx.x * kRowWarps + warp;
-  const int row = (int)(unit / per_row), part = (int)(unit % per_row);
+  constexpr int kLanes = D / 2 / V;     // lanes of a head row
+  constexpr int kHeads = 32 / kLanes;   // head rows a warp holds at once: a group
+  const int lane = threadIdx.x & 31;
+  const int heads = a.hq + a.hk + a.hv, groups = (heads + kHeads - 1) / kHeads;
+  const int parts = (groups + a.per_warp - 1) / a.per_warp;
+  const unsigned unit = blockIdx.x * kRowWarps + (threadIdx.x >> 5);
+  const int row = (int)(unit / parts), part = (int)(unit % parts);
   if (row >= a.rows) return;
-  const int sub = lane % kLanes, grp = lane / kLanes;
+  const int sub = lane % kLanes;
   const int e = sub * V;  // index of the lane's first pair
   const bool turned = e < a.r;
   const int lower = turned ? e : a.r + e;  // pairs past r: the untouched rest, split in halves
   const int upper = lower + (turned ? a.r : D / 2 - a.r);
+  const int first = part * a.per_warp, last = min(groups, first + a.per_warp);
 
-  // the rows' loads first: nothing they need depends on the position
-  uint4 lo[kIters], hi[kIters];
-#pragma unroll
-  for (int it = 0; it < kIters; ++it) {
-    const int h = (part * kIters + it) * kGroup_ + grp;
+  uint4 lo, hi;
+  auto load = [&](int it) {
+    const int h = it * kHeads + lane / kLanes;
+    lo = hi = make_uint4(0, 0, 0, 0);
     if (h < heads) {
       const T* src;
       if (h < a.hq)
@@ -182,12 +184,11 @@ __global__ void __launch_bounds__(32 * kRowWarps) rows_kernel(const RowArgs a) {
         src = static_cast<const T*>(a.k) + row * a.k_stride + (h - a.hq) * D;
       else
         src = static_cast<const T*>(a.v) + row * a.v_stride + (h - a.hq - a.hk) * D;
-      lo[it] = *reinterpret_cast<const uint4*>(src + lower);
-      hi[it] = *reinterpret_cast<const uint4*>(src + upper);
-    } else {
-      lo[it] = hi[it] = make_uint4(0, 0, 0, 0);
+      lo = *reinterpret_cast<const uint4*>(src + lower);
+      hi = *reinterpret_cast<const uint4*>(src + upper);
     }
-  }
+  };
+  load(first);  // nothing it needs depends on the position
 
   // where the row sits
   int p = 0;
@@ -234,13 +235,14 @@ __global__ void __launch_bounds__(32 * kRowWarps) rows_kernel(const RowArgs a) {
     }
   }
 
-#pragma unroll
-  for (int it = 0; it < kIters; ++it) {
-    const int h = (part * kIters + it) * kGroup_ + grp;
+#pragma unroll 1
+  for (int it = first; it < last; ++it) {
+    const int h = it * kHeads + lane / kLanes;
     const bool is_q = h < a.hq, is_v = h >= a.hq + a.hk;
     float x[V], y[V];
-    unpack(lo[it], x, T());
-    unpack(hi[it], y, T());
+    unpack(lo, x, T());
+    unpack(hi, y, T());
+    if (it + 1 < last) load(it + 1);
     const float* g = is_v ? nullptr : is_q ? a.q_gamma : a.k_gamma;
     if (a.q_gamma || a.k_gamma) {  // the same for the whole warp: the shuffles need every lane
       float ss = 0.0f;
@@ -249,7 +251,7 @@ __global__ void __launch_bounds__(32 * kRowWarps) rows_kernel(const RowArgs a) {
 #pragma unroll
       for (int o = kLanes / 2; o > 0; o >>= 1) ss = __fadd_rn(ss, __shfl_xor_sync(0xffffffffu, ss, o));
       if (g && h < heads) {
-        const float inv = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fmul_rn(ss, 1.0f / D), a.eps)));
+        const float inv = rsqrtf(__fadd_rn(__fmul_rn(ss, 1.0f / D), a.eps));
 #pragma unroll
         for (int i = 0; i < V; i += 4) {
           const float4 gl = __ldg(reinterpret_cast<const float4*>(g + lower + i));
