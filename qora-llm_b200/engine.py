@@ -359,8 +359,8 @@ def raw_prefill(weights: DecodeWeights, token_ids, max_seq: int = 4096):
 
 # ---------------------------------------------------------------- kernel entries
 def _stream_ptr(stream):
-    if stream is None:
-        return None
+    if stream is None or stream.__class__ is int:
+        return stream
     return int(getattr(stream, "cuda_stream", stream))
 
 
@@ -406,10 +406,10 @@ PAGED_WORK_BYTES = 64 << 20  # QORA_PAGED_WORK_BYTES
 
 
 def _dtype(name):
-    try:
-        return DTYPES[name]
-    except KeyError:
-        raise ValueError(f"element type {name!r}: one of {sorted(DTYPES)}") from None
+    dt = DTYPES.get(name)
+    if dt is None:
+        raise ValueError(f"element type {name!r}: one of {sorted(DTYPES)}")
+    return dt
 
 
 def qk_norm_rope(q_ptr, k_ptr, q_out_ptr, k_out_ptr, rows, q_heads, kv_heads, head_dim, pos_ptr, cos_ptr, sin_ptr,
@@ -418,11 +418,13 @@ def qk_norm_rope(q_ptr, k_ptr, q_out_ptr, k_out_ptr, rows, q_heads, kv_heads, he
     """RMSNorm of each head of q and k (with gains) and the rotation, in one pass
     (qora_qk_norm_rope). Strides are elements from one row to the next (default: no gap)."""
     nq, nk = q_heads * head_dim, kv_heads * head_dim
-    check(lib().qora_qk_norm_rope(
+    st = (_lib or lib()).qora_qk_norm_rope(
         q_ptr, nq if q_stride is None else q_stride, k_ptr, nk if k_stride is None else k_stride, _dtype(dtype), rows,
         q_heads, kv_heads, head_dim, q_gamma_ptr, k_gamma_ptr, eps, pos_ptr, cos_ptr, sin_ptr, rope_rows,
         rope_half_dim, q_out_ptr, nq if q_out_stride is None else q_out_stride, k_out_ptr,
-        nk if k_out_stride is None else k_out_stride, status_ptr, _stream_ptr(stream)))
+        nk if k_out_stride is None else k_out_stride, status_ptr, _stream_ptr(stream))
+    if st:
+        check(st)
 
 
 def paged_append(k_ptr, v_ptr, rows, kv_heads, head_dim, k_pages_ptr, v_pages_ptr, num_pages, page_size, q_start_ptr,
@@ -435,12 +437,14 @@ def paged_append(k_ptr, v_ptr, rows, kv_heads, head_dim, k_pages_ptr, v_pages_pt
     [page][head][slot][head_dim], the head-major order of KVCache."""
     nq, nk = q_heads * head_dim, kv_heads * head_dim
     ps, hs, ss = page_strides or (page_size * nk, page_size * head_dim, head_dim)
-    check(lib().qora_paged_append(
+    st = (_lib or lib()).qora_paged_append(
         q_ptr, nq if q_stride is None else q_stride, k_ptr, nk if k_stride is None else k_stride, v_ptr,
         nk if v_stride is None else v_stride, _dtype(dtype), rows, q_heads, kv_heads, head_dim, q_gamma_ptr,
         k_gamma_ptr, eps, cos_ptr, sin_ptr, rope_rows, rope_half_dim, q_out_ptr,
         nq if q_out_stride is None else q_out_stride, k_pages_ptr, v_pages_ptr, _dtype(kv_dtype), num_pages, page_size,
-        ps, hs, ss, q_start_ptr, kv_len_ptr, table_ptr, table_stride, seqs, status_ptr, _stream_ptr(stream)))
+        ps, hs, ss, q_start_ptr, kv_len_ptr, table_ptr, table_stride, seqs, status_ptr, _stream_ptr(stream))
+    if st:
+        check(st)
 
 
 def paged_attention(q_ptr, out_ptr, rows, q_heads, kv_heads, head_dim, k_pages_ptr, v_pages_ptr, num_pages, page_size,
@@ -451,11 +455,13 @@ def paged_attention(q_ptr, out_ptr, rows, q_heads, kv_heads, head_dim, k_pages_p
     scale: default 1 / sqrt(head_dim); page_strides as in paged_append."""
     nq, nk = q_heads * head_dim, kv_heads * head_dim
     ps, hs, ss = page_strides or (page_size * nk, page_size * head_dim, head_dim)
-    check(lib().qora_paged_attention(
+    st = (_lib or lib()).qora_paged_attention(
         q_ptr, nq if q_stride is None else q_stride, _dtype(dtype), rows, q_heads, kv_heads, head_dim,
         max(head_dim, 1) ** -0.5 if scale is None else scale, window, k_pages_ptr, v_pages_ptr, _dtype(kv_dtype), num_pages,
         page_size, ps, hs, ss, q_start_ptr, kv_len_ptr, table_ptr, table_stride, seqs, max_q, out_ptr,
-        nq if out_stride is None else out_stride, lse_ptr, work_ptr, work_bytes, status_ptr, _stream_ptr(stream)))
+        nq if out_stride is None else out_stride, lse_ptr, work_ptr, work_bytes, status_ptr, _stream_ptr(stream))
+    if st:
+        check(st)
 
 
 def tp_plan(fmt: int, num_heads: int, num_kv_heads: int, intermediate: int, vocab: int, tp: int, rank: int) -> dict:
