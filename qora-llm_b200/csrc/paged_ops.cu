@@ -130,7 +130,7 @@ qora_status allow_smem(int dev, int bytes) {
 
 // Fewest units of work worth a CTA of their own, and what a tile's fixed time counts, in steps.
 constexpr int kTokenMinSteps = 16;
-constexpr int kTokenTileCost = 16;
+constexpr int kTokenTileCost = 32;
 
 template <typename T, typename C, int D>
 qora_status launch_token(const paged::AttnArgs& a, void* work, cudaStream_t s) {

@@ -116,12 +116,17 @@ struct TokenCfg {
   QORA_DEV static int v_at(int row, int ch) { return row * kRowBytes + ((kWide ? ch ^ (row & 6) : ch ^ (row & 7)) << 4); }
   static constexpr int kSide = kPos * kRowBytes;  // bytes of a step's K (or V)
   static constexpr int kStep = 2 * kSide;
+  // q's fragments lie in shared memory, each warp makes a part of them: in registers they are
+  // 32 (f32 cache: 64) of a thread's, made by every warp for itself (32 tokens over f32
+  // caches: 61.5 us against 55.3 us)
   static constexpr int kStages = 3;
   static constexpr int kWarps = 8;
+  static constexpr int kQSteps = D / (kWide ? 8 : 16);  // k steps of a score
+  static constexpr int kQBytes = kQSteps * 32 * 16;
   static constexpr int kRing = kStages * kStep;  // bytes of a warp's ring
   static constexpr int kNum = D + (kWide ? 4 : 8);  // floats from one row of numerators to the next, in the ring
   static_assert(kRows * kNum * 4 <= kRing, "the ring holds the numerators");
-  static constexpr int kSmem = kWarps * kRing;
+  static constexpr int kSmem = kWarps * kRing + kQBytes;
 };
 
 constexpr int kTokenMaxCtas = 320;
@@ -183,6 +188,7 @@ __global__ void __launch_bounds__(32 * TokenCfg<T, C, D>::kWarps, 1) token_kerne
   using Cfg = TokenCfg<T, C, D>;
   constexpr int kPos = Cfg::kPos, kRows = Cfg::kRows, kWarps = Cfg::kWarps, kChunks = Cfg::kChunks, kStages = Cfg::kStages;
   constexpr bool kWide = Cfg::kWide, kHalves = Cfg::kHalves;
+  static_assert(D / 16 <= kWarps, "a warp for each part of q");
   constexpr int kThr = 32 * kWarps;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float2 s_ml[kWarps][kRows];
@@ -317,52 +323,57 @@ __global__ void __launch_bounds__(32 * TokenCfg<T, C, D>::kWarps, 1) token_kerne
 
     // q in the instruction's layout. f32 rows: 2^e puts the row's largest value in [2^13, 2^14)
     float qscale[2] = {scale2, scale2};
-    constexpr int kQ = kWide ? D / 8 : D / 16;
-    uint32_t qa[kQ][4];
+    uint4* const s_q = reinterpret_cast<uint4*>(smem + kWarps * Cfg::kRing);  // [k step][lane]
     auto row_ptr = [&](int r) {
       const int tok = token_of(a, r);
       return static_cast<const T*>(a.q) + (long long)(sw.q0 + tok) * a.q_stride + (head * a.group + r - tok * a.group) * D;
     };
-    float qx[kHalves ? 2 * D / 8 : 1];  // f32 rows as loaded; the loads are under way while the first copies are issued
+    // the loads are under way while the first copies are issued
+    uint32_t qw[4];        // 16-bit rows: the warp's k step; f32 rows: the thread's dims of it
+    float mx = 0.0f;       // f32 rows, 16-bit cache: the row's largest value
     if constexpr (!kHalves) {
+      if (warp < Cfg::kQSteps) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const bool ok = g + 8 * i < nrows;
-        const T* q = row_ptr(ok ? g + 8 * i : 0);
-#pragma unroll
-        for (int k = 0; k < kQ; ++k) {
-          qa[k][i] = ok ? *reinterpret_cast<const uint32_t*>(q + 16 * k + 2 * t) : 0u;
-          qa[k][2 + i] = ok ? *reinterpret_cast<const uint32_t*>(q + 16 * k + 8 + 2 * t) : 0u;
+        for (int i = 0; i < 2; ++i) {
+          const bool ok = g + 8 * i < nrows;
+          const T* q = row_ptr(ok ? g + 8 * i : 0) + 16 * warp + 2 * t;
+          qw[i] = ok ? *reinterpret_cast<const uint32_t*>(q) : 0u;
+          qw[2 + i] = ok ? *reinterpret_cast<const uint32_t*>(q + 8) : 0u;
         }
       }
     } else {
-      const float* q = reinterpret_cast<const float*>(row_ptr(g < nrows ? g : 0));
-      constexpr int kV = kWide ? 4 : 2;  // floats of a load: 16 b + 4 t.. or 8 k + 2 t..
+      const bool ok = g < nrows;
+      const float* q = reinterpret_cast<const float*>(row_ptr(ok ? g : 0));
+      if (warp < D / 16) {
+        // two k steps of 8: dims 16 b + 4 t ..; one of 16: 16 k + 2 t .. and 8 on
+        const float2 u = *reinterpret_cast<const float2*>(q + 16 * warp + (kWide ? 4 : 2) * t);
+        const float2 v = *reinterpret_cast<const float2*>(q + 16 * warp + (kWide ? 4 * t + 2 : 2 * t + 8));
+        qw[0] = ok ? __float_as_uint(u.x) : 0u;
+        qw[1] = ok ? __float_as_uint(u.y) : 0u;
+        qw[2] = ok ? __float_as_uint(v.x) : 0u;
+        qw[3] = ok ? __float_as_uint(v.y) : 0u;
+      }
+      if constexpr (!kWide) {
 #pragma unroll
-      for (int k = 0; k < D / 4 / kV; ++k)
-#pragma unroll
-        for (int j = 0; j < kV; j += 2) {
-          const float2 y = *reinterpret_cast<const float2*>(q + 4 * kV * k + kV * t + j);
-          qx[kV * k + j] = y.x;
-          qx[kV * k + j + 1] = y.y;
+        for (int k = 0; k < D / 16; ++k) {
+          const float4 u = *reinterpret_cast<const float4*>(q + 16 * k + 4 * t);
+          mx = fmaxf(mx, fmaxf(fmaxf(fabsf(u.x), fabsf(u.y)), fmaxf(fabsf(u.z), fabsf(u.w))));
         }
+        if (!ok) mx = 0.0f;
+      }
     }
     auto make_q = [&]() {
-      if constexpr (kHalves) {
-        if (g >= nrows) {
-#pragma unroll
-          for (int k = 0; k < D / 4; ++k) qx[k] = 0.0f;
-        }
+      if constexpr (!kHalves) {
+        if (warp < Cfg::kQSteps) s_q[warp * 32 + lane] = make_uint4(qw[0], qw[1], qw[2], qw[3]);
+      } else {
+        const float x[4] = {__uint_as_float(qw[0]), __uint_as_float(qw[1]), __uint_as_float(qw[2]), __uint_as_float(qw[3])};
         if constexpr (kWide) {  // tf32: the exponent range is f32's, no scale
+          if (warp < D / 16) {
 #pragma unroll
-          for (int k = 0; k < D / 4; ++k) {
-            qa[k >> 1][2 * (k & 1)] = tf32_hi(qx[k]);
-            qa[k >> 1][2 * (k & 1) + 1] = tf32_lo(qx[k]);
+            for (int k = 0; k < 2; ++k)
+              s_q[(2 * warp + k) * 32 + lane] = make_uint4(tf32_hi(x[2 * k]), tf32_lo(x[2 * k]), tf32_hi(x[2 * k + 1]), tf32_lo(x[2 * k + 1]));
           }
         } else {
-          float mx = 0.0f;
-#pragma unroll
-          for (int k = 0; k < D / 4; ++k) mx = fmaxf(mx, fabsf(qx[k]));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
           // exponent of mx (0 for zeros and subnormals, 255 for non-finite rows: no scale)
@@ -370,16 +381,20 @@ __global__ void __launch_bounds__(32 * TokenCfg<T, C, D>::kWarps, 1) token_kerne
           const int up = ex == 0 || ex == 255 ? 0 : min(126, 140 - ex);
           const float mul = __uint_as_float((uint32_t)(127 + up) << 23);
           qscale[0] = scale2 * __uint_as_float((uint32_t)(127 - up) << 23);
+          if (warp < D / 16) {
+            uint32_t w[4];
 #pragma unroll
-          for (int k = 0; k < D / 8; ++k) {
-            const float u = qx[2 * k] * mul, v = qx[2 * k + 1] * mul;
-            const uint32_t hi = pack2(u, v, __half());
-            const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&hi));
-            qa[k >> 1][2 * (k & 1)] = hi;
-            qa[k >> 1][2 * (k & 1) + 1] = pack2(u - h.x, v - h.y, __half());
+            for (int k = 0; k < 2; ++k) {
+              const float u = x[2 * k] * mul, v = x[2 * k + 1] * mul;
+              w[2 * k] = pack2(u, v, __half());
+              const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&w[2 * k]));
+              w[2 * k + 1] = pack2(u - h.x, v - h.y, __half());
+            }
+            s_q[warp * 32 + lane] = make_uint4(w[0], w[1], w[2], w[3]);
           }
         }
       }
+      __syncthreads();
     };
 
     constexpr int kO = D / 8;  // numerators: n8 tiles of 4 values
@@ -428,28 +443,37 @@ __global__ void __launch_bounds__(32 * TokenCfg<T, C, D>::kWarps, 1) token_kerne
         constexpr int kN = kPos / 8;
         float s[kN][4];
         if constexpr (kWide) {
-          float u[4] = {0.0f, 0.0f, 0.0f, 0.0f}, v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+          float u[4] = {}, v[4] = {}, u2[4] = {}, v2[4] = {};
 #pragma unroll
           for (int b = 0; b < D / 16; ++b) {
             const float4 k = *reinterpret_cast<const float4*>(pk + Cfg::k_at(g, 4 * b + t));
-            mma_tf32(u, qa[2 * b], tf32_hi(k.x), tf32_hi(k.y));
-            mma_tf32(v, qa[2 * b], tf32_lo(k.x), tf32_lo(k.y));
-            mma_tf32(u, qa[2 * b + 1], tf32_hi(k.z), tf32_hi(k.w));
-            mma_tf32(v, qa[2 * b + 1], tf32_lo(k.z), tf32_lo(k.w));
+            const uint4 q0 = s_q[(2 * b) * 32 + lane], q1 = s_q[(2 * b + 1) * 32 + lane];
+            const uint32_t a0[4] = {q0.x, q0.y, q0.z, q0.w}, a1[4] = {q1.x, q1.y, q1.z, q1.w};
+            mma_tf32(u, a0, tf32_hi(k.x), tf32_hi(k.y));
+            mma_tf32(v, a0, tf32_lo(k.x), tf32_lo(k.y));
+            mma_tf32(u2, a1, tf32_hi(k.z), tf32_hi(k.w));
+            mma_tf32(v2, a1, tf32_lo(k.z), tf32_lo(k.w));
           }
 #pragma unroll
-          for (int j = 0; j < 4; ++j) s[0][j] = u[j] + v[j];
+          for (int j = 0; j < 4; ++j) s[0][j] = (u[j] + u2[j]) + (v[j] + v2[j]);
         } else {
 #pragma unroll
           for (int n = 0; n < kN; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
+          float s2[kN][4] = {};  // two sums each: shorter chains
           const int mi = lane >> 3, row = (mi >> 1) * 8 + (lane & 7);
 #pragma unroll
-          for (int k = 0; k < kQ; ++k) {
+          for (int k = 0; k < Cfg::kQSteps; ++k) {
             uint32_t b[4];
             ldsm4(b, sk + Cfg::k_at(row, 2 * k + (mi & 1)));
-            mma16(s[0], qa[k], b[0], b[1], C());
-            mma16(s[1], qa[k], b[2], b[3], C());
+            const uint4 q4 = s_q[k * 32 + lane];
+            const uint32_t qa[4] = {q4.x, q4.y, q4.z, q4.w};
+            mma16(k & 1 ? s2[0] : s[0], qa, b[0], b[1], C());
+            mma16(k & 1 ? s2[1] : s[1], qa, b[2], b[3], C());
           }
+#pragma unroll
+          for (int n = 0; n < kN; ++n)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s[n][j] += s2[n][j];
         }
         constexpr int kR = kHalves ? 1 : 2;
         if constexpr (kHalves) {
