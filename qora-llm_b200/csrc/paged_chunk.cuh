@@ -37,9 +37,10 @@
 // The running maximum is raised only when it grows by more than 2^kSlack: then the
 // numerators in TMEM are scaled, which is rare after the first tiles. Masked scores become
 // -inf before the maximum. Rows that meet a non-finite value (a weight of zero times an
-// infinite value of V, or a row whose own scores are), and rows of a cache whose tiles of V
-// differ by more than 2^12 in size, are computed again by one warp, one position at a time
-// (row_attend).
+// infinite value of V, or a row whose own scores are) are computed again by one warp, one
+// position at a time (row_attend). So are rows of an f32 cache that meet a tile of K or V
+// whose rows differ by more than 2^14 in size, a tile of V 2^12 below the largest before
+// it, or growth of V by more than 2^60.
 #pragma once
 
 #include <cuda.h>
@@ -329,6 +330,10 @@ QORA_DEV void split4(const float4& x, float mul, uint2& hi, uint2& lo) {
 QORA_DEV int scale_up(uint32_t bits) { return min(126, 140 - (int)(bits >> 23)); }
 QORA_DEV float pow2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
 constexpr int kNoScale = 127;  // a tile of zeros
+// Two halves of a value 2^-kMaxSpread of the tile's largest still have 22 bits; weights that
+// are scaled down by 2^kMaxLift have 20 or more. Numerators that were scaled down by
+// 2^kMaxDrop are still far from f32's subnormals. Beyond that the rows are computed again.
+constexpr int kMaxSpread = 14, kMaxLift = 12, kMaxDrop = 60, kSpreadMark = 1024;
 
 // byte offset of 16-byte piece `piece` of a row in a tile whose 64-element halves are `half` bytes apart
 QORA_DEV int tile_at(int row, int piece, int half) { return (piece >> 3) * half + row * 128 + (((piece & 7) ^ (row & 7)) << 4); }
@@ -358,7 +363,8 @@ __global__ void __launch_bounds__(ChunkCfg<T, C, D>::kThreads, 1)
   uint32_t* const s_bad = reinterpret_cast<uint32_t*>(bars + 26);  // [8 tiles][4] positions that there are not
   int* const s_exp = reinterpret_cast<int*>(s_bad + 32);           // [8 tiles][K, V] scales of the tiles
   uint32_t* const s_max = reinterpret_cast<uint32_t*>(s_exp + 16);  // [K, V][4 warps]
-  uint32_t* const s_tmem = s_max + 8;
+  uint32_t* const s_low = s_max + 8;                                // [K, V][4 warps]
+  uint32_t* const s_tmem = s_low + 8;
   volatile int* const abort_flag = reinterpret_cast<volatile int*>(s_tmem + 1);
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -646,20 +652,32 @@ __global__ void __launch_bounds__(ChunkCfg<T, C, D>::kThreads, 1)
             const uint32_t b = __float_as_uint(v) & 0x7FFFFFFFu;
             return b < 0x7F800000u ? b : 0u;
           };
+          // the largest magnitude of the tile, and of its smallest row that is not zero
+          uint32_t low = 0xffffffffu;
+          const unsigned row_lanes = kF4 == 32 ? 0xffffffffu : lane < 16 ? 0xffffu : 0xffff0000u;
 #pragma unroll
-          for (int i = 0; i < kN; ++i)
-            mx = max(max(mx, max(finite_bits(x[i].x), finite_bits(x[i].y))), max(finite_bits(x[i].z), finite_bits(x[i].w)));
+          for (int i = 0; i < kN; ++i) {
+            uint32_t of_row = max(max(finite_bits(x[i].x), finite_bits(x[i].y)), max(finite_bits(x[i].z), finite_bits(x[i].w)));
+            of_row = __reduce_max_sync(row_lanes, of_row);
+            mx = max(mx, of_row);
+            if (of_row) low = min(low, of_row);
+          }
           mx = __reduce_max_sync(0xffffffffu, mx);
+          low = __reduce_min_sync(0xffffffffu, low);
           if (lane == 0) s_max[team * 4 + lw] = mx;
+          if (lane == 0) s_low[team * 4 + lw] = low;
           const uint32_t st = entry % kStages;
           const bool free = wait(empty + st, ((entry / kStages) & 1) ^ 1);
           ok = ok && free;
           ptx::named_bar(bar_id, kLoaders);
           const uint4 m4 = *reinterpret_cast<const uint4*>(s_max + team * 4);
+          const uint4 l4 = *reinterpret_cast<const uint4*>(s_low + team * 4);
           mx = max(max(m4.x, m4.y), max(m4.z, m4.w));
+          low = min(min(l4.x, l4.y), min(l4.z, l4.w));
           const int up = mx ? scale_up(mx) : kNoScale;
+          const bool spread = mx && (int)(mx >> 23) - (int)(low >> 23) > kMaxSpread;
           const float mul = mx ? pow2(up) : 1.0f;
-          if (lt == 0) s_exp[ring8 * 2 + team] = up;
+          if (lt == 0) s_exp[ring8 * 2 + team] = up + (spread ? kSpreadMark : 0);
           uint8_t* dst = ring + st * Cfg::kStage;
           if (ok) {
 #pragma unroll
@@ -750,7 +768,7 @@ __global__ void __launch_bounds__(ChunkCfg<T, C, D>::kThreads, 1)
         }
       }
       float m = -INFINITY, l = 0.0f;
-      int e_ref = kNoScale;  // f32 cache: the numerators count in 2^-e_ref
+      int e_ref = kNoScale, e_first = kNoScale;  // f32 cache: the numerators count in 2^-e_ref
       bool wild = false;
       // f32 rows: numerators of earlier tiles, relative to m_acc and e_acc, in the workspace
       float m_acc = -INFINITY;
@@ -803,14 +821,18 @@ __global__ void __launch_bounds__(ChunkCfg<T, C, D>::kThreads, 1)
             const uint32_t ev = (tiles + j) * 2 + 1;  // V's scale: its tile stays until this block's weights are used
             ok = wait_all(full + ev % kStages, (ev / kStages) & 1);
             if (!ok) break;
-            const int ek = s_exp[ring8 * 2], eV = s_exp[ring8 * 2 + 1];
+            int ek = s_exp[ring8 * 2], eV = s_exp[ring8 * 2 + 1];
+            wild |= ek > kSpreadMark / 2 || eV > kSpreadMark / 2;
+            if (ek > kSpreadMark / 2) ek -= kSpreadMark;
+            if (eV > kSpreadMark / 2) eV -= kSpreadMark;
             if (ek != kNoScale) ct = c * pow2(-ek);
             if (eV != kNoScale) {
               if (eV < e_ref) {
                 if (e_ref != kNoScale) o_scale = pow2(max(-126, eV - e_ref));
+                else e_first = eV;
                 e_ref = eV;
               }
-              wild |= eV - e_ref > 12;
+              wild |= eV - e_ref > kMaxLift || e_first - e_ref > kMaxDrop;
               lift = (float)(e_ref - eV);
               l_scale = pow2(min(126, eV - e_ref));
             }

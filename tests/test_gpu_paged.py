@@ -423,35 +423,115 @@ def test_attention_infinite_values_reach_only_rows_that_see_them(pkg, torch, t, 
     assert np.all(np.isnan(got[1, 0])) and np.isfinite(got[0]).all() and np.isfinite(got[2:n]).all() and np.isfinite(got[1, 1:]).all()
 
 
+def check_on_gpu(torch, b, got, gl, q, pool, t, kv, window=0):
+    """check_attention in 64 bits on the GPU, for more positions than numpy loops take."""
+    hq, d, hk = q.shape[1], q.shape[2], pool.hk
+    for s in range(b.seqs):
+        L, n = b.total[s], b.new[s]
+        pg = torch.from_numpy(b.table[s, :-(-L // b.page)].astype(np.int64)).cuda()
+        k, v = (z.double()[pg][..., :d] for z in pool.t)
+        k, v = ((z if pool.layout == "slot" else z.transpose(1, 2)).reshape(-1, hk, d)[:L] for z in (k, v))
+        p, j = torch.arange(L - n, L, device="cuda")[:, None], torch.arange(L, device="cuda")[None]
+        hide = (j > p) | (j <= p - window) if window else j > p
+        for h in range(hq):
+            rows, g = slice(b.start[s], b.start[s] + n), h // (hq // hk)
+            x = torch.from_numpy(q[rows, h]).cuda() @ k[:, g].T * d ** -0.5
+            x[hide] = -np.inf
+            w = torch.softmax(x, 1)
+            out, mass = (w @ v[:, g]).cpu().numpy(), (w @ v[:, g].abs()).cpu().numpy()
+            size = (torch.from_numpy(np.abs(q[rows, h])).cuda() @ k[:, g].abs().T * d ** -0.5).masked_fill(hide, 0).amax(1).cpu().numpy()
+            bound, lb = ref.attention_bounds(b, out, mass, size, t, kv, d)
+            err = np.abs(got[rows, h] - out)
+            assert np.all(err <= bound), (s, h, float(np.max(err / bound)))
+            wl = torch.logsumexp(x, 1).cpu().numpy()
+            assert np.all(np.abs(gl[rows, h] - wl) <= lb + 2.0**-23 * np.abs(wl))
+
+
 @pytest.mark.parametrize("t,kv", TYPES)
-@pytest.mark.parametrize("n", [1, 40])
-def test_attention_longer_caches(pkg, torch, t, kv, n):
-    """Work split over the positions: thousands of them, two sequences of very different
-    length, against 64 bits on the GPU."""
-    g = torch.Generator(device="cuda").manual_seed(n)
-    page, hq, hk, d, total = 16, 8, 2, 128, [9001, 300]
-    b = ref.Batch(np.random.default_rng(1), [n, n], total, page)
-    pool = Pool(torch, kv, b, hk, d, "slot")
+@pytest.mark.parametrize("new,total,page,layout,hq,hk,d,window", [
+    ([1, 1], [9001, 300], 16, "slot", 8, 2, 128, 0),               # split over the positions
+    ([40, 40], [9001, 300], 16, "slot", 8, 2, 128, 0),
+    ([70] * 20, [1500 - 61 * s for s in range(20)], 64, "head", 16, 4, 128, 0),  # many tiles in one piece
+    ([33, 1, 200, 7] * 10, [700, 1300, 410, 900] * 10, 32, "slot", 8, 4, 64, 0),
+    ([90] * 16, [1200] * 16, 128, "slot", 16, 4, 64, 500),         # pages longer than a tile
+    ([90] * 16, [900] * 16, 24, "head", 12, 4, 128, 333),          # pages that no tile is made of
+    ([600], [600], 256, "head", 6, 2, 128, 0),
+    ([2] * 40, [31 * s + 2 for s in range(40)], 16, "head", 8, 2, 128, 0),
+])
+def test_attention_longer_caches(pkg, torch, t, kv, new, total, page, layout, hq, hk, d, window):
+    """Work split over the positions, and pieces of many tiles, against 64 bits on the GPU."""
+    g = torch.Generator(device="cuda").manual_seed(len(new))
+    b = ref.Batch(np.random.default_rng(1), new, total, page)
+    pool = Pool(torch, kv, b, hk, d, layout)
     for z in pool.t:
         z.copy_(torch.randn(z.shape, generator=g, device="cuda"))
     q = ref.round_to(np.random.default_rng(2).standard_normal((b.rows, hq, d)) * 1.5, t)
+    got, gl, st = attend(pkg, torch, b, q, pool, t, window=window)
+    assert st == 0
+    check_on_gpu(torch, b, got, gl, q, pool, t, kv, window)
+
+
+@pytest.mark.parametrize("n,seqs", [(1, 2), (40, 1), (70, 20)])
+@pytest.mark.parametrize("qs,ks,vs", [(1e-15, 1e15, 1.0), (1e12, 1e-12, 1e-30), (1.0, 1.0, 1e30), (1.0, 1.0, "steps"),
+                                      (1.0, 1.0, "late"), (1.0, "steps", 1.0), (1.0, 1.0, "zeros"), (1.0, 1.0, "far"),
+                                      (1.0, 1.0, "grows")])
+def test_attention_f32_cache_of_any_size(pkg, torch, n, seqs, qs, ks, vs):
+    """f32 caches whose values lie far from 1, or whose tiles differ in size: "steps": every 64
+    positions another magnitude, "late": large values at the end alone, "zeros": tiles of zeros,
+    "far": late values that are 1e45 times as large, "grows": 1000 times as large every 64."""
+    g = torch.Generator(device="cuda").manual_seed(n)
+    total = [900 + s for s in range(seqs)]
+    b = ref.Batch(np.random.default_rng(1), [n] * seqs, total, 16)
+    pool = Pool(torch, "f32", b, 4, 128, "slot")
+    size = {"steps": lambda p: 10.0 ** (3.0 * ((p // 64) % 5) - 8), "late": lambda p: np.where(p < 850, 1.0, 1e9),
+            "zeros": lambda p: np.where((p // 64) % 3 == 0, 0.0, 1.0),
+            "far": lambda p: np.where(p < 832 + 64 * (p[-1] > 910), 1e-20, 1e25), "grows": lambda p: 10.0 ** (3.0 * (p // 64) - 20)}
+    for z, f in zip(pool.t, (ks, vs)):
+        z.copy_(torch.randn(z.shape, generator=g, device="cuda"))
+        for s in range(seqs):
+            p = np.arange(total[s])
+            f_p = size[f](p) if isinstance(f, str) else np.full(total[s], f)
+            pg = torch.from_numpy(b.table[s, p // 16].astype(np.int64)).cuda()
+            z[pg, torch.from_numpy(p % 16).cuda()] *= torch.from_numpy(f_p).float().cuda()[:, None, None]
+    q = ref.round_to(np.random.default_rng(2).standard_normal((b.rows, 16, 128)) * qs * (1e-3 if ks == "steps" else 1.0), "f32")
+    got, gl, st = attend(pkg, torch, b, q, pool, "f32")
+    assert st == 0
+    check_on_gpu(torch, b, got, gl, q, pool, "f32", "f32")
+
+
+@pytest.mark.parametrize("qs", [1e-30, 1e-6, 1e6, 3e30])
+@pytest.mark.parametrize("n", [1, 40])
+def test_attention_f32_rows_of_any_size(pkg, torch, n, qs):
+    rng = np.random.default_rng(4)
+    b, q, pages, pool = make(torch, rng, "f32", "f16", [n], [200], 16, "slot", 4, 1, 64, extra=0)
+    q = ref.round_to(q * qs, "f32")
+    scale = float(np.float32(0.125 / qs)) if qs != 1e-30 else 0.125
+    got, gl, st = attend(pkg, torch, b, q, pool, "f32", scale=scale)
+    check_attention(b, got, gl, q, pages, "f32", "f16", scale, 0)
+
+
+@pytest.mark.parametrize("t,kv", TYPES)
+@pytest.mark.parametrize("n", [1, 30])
+def test_attention_of_sequences_that_share_pages(pkg, torch, t, kv, n):
+    rng = np.random.default_rng(6)
+    b, q, pages, pool = make(torch, rng, t, kv, [n] * 3, [100, 90, 64], 16, "head", 4, 2, 64)
+    b.table[1, :4], b.table[2, :4] = b.table[0, :4], b.table[0, :4]
     got, gl, st = attend(pkg, torch, b, q, pool, t)
     assert st == 0
-    for s in range(2):
-        pg = torch.from_numpy(b.table[s, :-(-total[s] // page)].astype(np.int64)).cuda()
-        k, v = (z.double()[pg].reshape(-1, hk, d)[:total[s]] for z in pool.t)
-        for h in range(hq):
-            rows = slice(b.start[s], b.start[s] + n)
-            x = torch.from_numpy(q[rows, h]).cuda() @ k[:, h // 4].T * d ** -0.5
-            p = torch.arange(total[s] - n, total[s], device="cuda")[:, None]
-            x[torch.arange(total[s], device="cuda")[None] > p] = -np.inf
-            w = torch.softmax(x, 1)
-            out, mass = (w @ v[:, h // 4]).cpu().numpy(), (w @ v[:, h // 4].abs()).cpu().numpy()
-            size = (torch.from_numpy(np.abs(q[rows, h])).cuda() @ k[:, h // 4].abs().T * d ** -0.5).amax(1).cpu().numpy()
-            bound, lb = ref.attention_bounds(b, out, mass, size, t, kv, d)
-            assert np.all(np.abs(got[rows, h] - out) <= bound)
-            wl = torch.logsumexp(x, 1).cpu().numpy()
-            assert np.all(np.abs(gl[rows, h] - wl) <= lb + 2.0**-23 * np.abs(wl))
+    check_attention(b, got, gl, q, pages, t, kv, 0.125, 0)
+
+
+@pytest.mark.parametrize("t,kv", TYPES)
+def test_attention_overlapping_row_ranges_stay_in_bounds(pkg, torch, t, kv):
+    """Row ranges that fall back: more tiles than the rows can have. Nothing is written."""
+    rng = np.random.default_rng(7)
+    b, q, pages, pool = make(torch, rng, t, kv, [320, 320], [320, 320], 16, "slot", 2, 1, 64, extra=0)
+    b.start = np.array([0, 640, 0, 640, 0, 640, 0, 640, 0], np.int32)
+    b.seqs, b.len = 8, np.full(8, 640, np.int32)
+    b.table = np.tile(np.arange(40, dtype=np.int32), (8, 1))
+    b.wide, b.new = 40, [640] * 8
+    got, gl, st = attend(pkg, torch, b, q, pool, t)
+    assert st == RANGE and np.all(got == -7.0) and np.all(gl == -7.0)
 
 
 def test_attention_page_offsets_past_32_bits(pkg, torch):
