@@ -88,7 +88,7 @@ constexpr int kChunkMaxCtas = 160;
 constexpr unsigned long long kWaitNs = 2000000000ull;
 
 constexpr int kChunkMaxParts = kChunkMaxCtas;  // parts of split items in one call: no more than CTAs
-// Workspace of split items: [tile and head] (first row, tokens, kv head), [part] (maximum,
+// Workspace of split items: [tile and head] (first row, tokens, kv head, parts), [part] (maximum,
 // sum) of 256 rows, numerators [part][256][D].
 __host__ __device__ inline int4* chunk_rec(void* p) { return static_cast<int4*>(p); }
 __host__ __device__ inline float2* chunk_ml(void* p) {
@@ -340,7 +340,7 @@ QORA_DEV int tile_at(int row, int piece, int half) { return (piece >> 3) * half 
 
 template <typename T, typename C, int D>
 __global__ void __launch_bounds__(ChunkCfg<T, C, D>::kThreads, 1)
-    chunk_kernel(const AttnArgs a, void* work, int splits, int max_items, int box_rows,
+    chunk_kernel(const AttnArgs a, void* work, bool split, int max_tiles, int box_rows,
                  const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
                  const __grid_constant__ CUtensorMap vmap) {
   using Cfg = ChunkCfg<T, C, D>;
@@ -392,13 +392,14 @@ __global__ void __launch_bounds__(ChunkCfg<T, C, D>::kThreads, 1)
   __syncthreads();
   umma::tc_fence_after();
   const uint32_t tmem = *s_tmem;
-  // more row tiles than the rows can hold: the sequences' row ranges overlap
-  const bool too_many = (long long)map.total * a.hk * splits > max_items;
-  if (too_many && tid == 0 && a.status) *a.status = 5u;
-  const int items = too_many ? 0 : map.total * a.hk * splits;
   const int ctas = (int)gridDim.x, cta = (int)blockIdx.x;
-  if (splits > 1 && cta == 0) {  // no rows for the join in the tiles that there are not
-    for (int i = items / splits + tid; i < max_items / splits; i += Cfg::kThreads) chunk_rec(work)[i] = make_int4(0, 0, 0, 0);
+  // more row tiles than the rows can hold: the sequences' row ranges overlap
+  const bool too_many = (long long)map.total * a.hk > max_tiles;
+  if (too_many && tid == 0 && a.status) *a.status = 5u;
+  const int whole = too_many ? 0 : map.total * a.hk;
+  const int splits = split && whole ? max(1, ctas / whole) : 1, items = whole * splits;
+  if (split && cta == 0) {  // no rows for the join where there is nothing to join
+    for (int i = (splits > 1 ? whole : 0) + tid; i < max_tiles; i += Cfg::kThreads) chunk_rec(work)[i] = make_int4(0, 0, 0, 0);
   }
   // item of turn w: alternating direction, so that long and short items pair up
   auto item_of = [&](int w) { return w * ctas + (w & 1 ? ctas - 1 - cta : cta); };
@@ -720,7 +721,7 @@ __global__ void __launch_bounds__(ChunkCfg<T, C, D>::kThreads, 1)
       const bool busy = toks > 0 && it.tiles > 0;
       const long long row0 = it.q0 + it.tok0 + x * block_toks;  // the block's first row
       if (it.part >= 0 && idx % splits == 0 && tid == 0)
-        chunk_rec(work)[idx / splits] = make_int4((int)row0, it.toks, it.head, 0);
+        chunk_rec(work)[idx / splits] = make_int4((int)row0, it.toks, it.head, splits);
       float c = scale2;
       if constexpr (kHalves) {
         // the warp's rows of q, eight at a time: four lanes a row, every fourth float4 each.
@@ -1048,10 +1049,11 @@ __global__ void __launch_bounds__(ChunkCfg<T, C, D>::kThreads, 1)
 
 // Split items: a warp adds the parts of a row in order; block (tile and head, group of 8 rows).
 template <typename T, int D>
-__global__ void __launch_bounds__(256) chunk_join_kernel(const AttnArgs a, void* work, int splits) {
+__global__ void __launch_bounds__(256) chunk_join_kernel(const AttnArgs a, void* work) {
   constexpr int E = D / 32, kAhead = 8;
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int4 rec = chunk_rec(work)[blockIdx.x];  // (first row, tokens, kv head)
+  const int4 rec = chunk_rec(work)[blockIdx.x];  // (first row, tokens, kv head, parts)
+  const int splits = rec.w;
   const int lane = threadIdx.x & 31, rr = blockIdx.y * 8 + (threadIdx.x >> 5), x = rr >> 7, r = rr & 127;
   const int block_toks = 128 / a.group, rtok = row_token(a, r), tok = x * block_toks + rtok;
   if (rtok >= block_toks || tok >= rec.y) return;

@@ -191,12 +191,13 @@ qora_status launch_chunk(const paged::AttnArgs& a, void* work, cudaStream_t s) {
   QCHECK((allow_smem<&paged::chunk_kernel<T, C, D>>(dev, Cfg::kSmem)));
   const int sms = std::min(sm_count(dev), paged::kChunkMaxCtas);
   const int block_toks = Cfg::kBlock / a.group, tokens = 2 * block_toks;
-  // row tiles that sequences with disjoint rows can have; items of long caches are split
-  // until there is one for every SM
+  // row tiles that sequences with disjoint rows can have, and that they are likely to have.
+  // Where those leave half of the SMs idle, the kernel splits the items of long caches
   const long long most = ((long long)a.batch.rows + (long long)a.batch.seqs * (tokens - 1)) / tokens * a.hk;
-  if (most > 0x7fffffff / sms) return fail(QORA_ERR_INVALID, "%d rows of %d sequences", a.batch.rows, a.batch.seqs);
-  const int splits = most >= sms ? 1 : (int)(sms / most);
-  const int ctas = (int)std::min<long long>(sms, most * splits);
+  const long long likely = ((long long)a.batch.rows + (long long)a.batch.seqs * (tokens / 2)) / tokens * a.hk;
+  if (most > 0x7fffffff) return fail(QORA_ERR_INVALID, "%d rows of %d sequences", a.batch.rows, a.batch.seqs);
+  const bool split = 2 * likely <= sms && most <= paged::kChunkMaxParts;
+  const int ctas = split ? sms : (int)std::min<long long>(sms, most);
   CUtensorMap qmap{}, kmap{}, vmap{};
   int box_rows = 0;
   if constexpr (!Cfg::kWide) {
@@ -212,10 +213,9 @@ qora_status launch_chunk(const paged::AttnArgs& a, void* work, cudaStream_t s) {
     const cuuint32_t box[3] = {64, (cuuint32_t)a.group, (cuuint32_t)block_toks};
     if (!encode_rows<T>(&qmap, a.q, 3, dims, strides, box)) return fail(QORA_ERR_CUDA, "cuTensorMapEncodeTiled failed on q");
   }
-  paged::chunk_kernel<T, C, D><<<ctas, Cfg::kThreads, Cfg::kSmem, s>>>(a, work, splits, (int)(most * splits), box_rows,
-                                                                      qmap, kmap, vmap);
+  paged::chunk_kernel<T, C, D><<<ctas, Cfg::kThreads, Cfg::kSmem, s>>>(a, work, split, (int)most, box_rows, qmap, kmap, vmap);
   QCUDA(cudaGetLastError());
-  if (splits == 1) return QORA_OK;
+  if (!split) return QORA_OK;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)most, a.max_q > block_toks ? 32 : 16);
   cfg.blockDim = dim3(256);
@@ -225,7 +225,7 @@ qora_status launch_chunk(const paged::AttnArgs& a, void* work, cudaStream_t s) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  QCUDA(cudaLaunchKernelEx(&cfg, paged::chunk_join_kernel<T, D>, a, work, splits));
+  QCUDA(cudaLaunchKernelEx(&cfg, paged::chunk_join_kernel<T, D>, a, work));
   return QORA_OK;
 }
 
