@@ -5,10 +5,14 @@
 // Item. Two blocks (X = 0, 1) of up to 128 packed rows of one (sequence, kv head): tokens
 // times the kv head's query heads (row r: token r / group, head r % group), so that grouped
 // heads share every K and V tile. Each block has its scores and its numerators (D columns)
-// in TMEM; K and V tiles of 128 positions (64 of an f32 cache) feed both. Where there are
-// few items, the positions of an item are split evenly and chunk_join_kernel adds the parts
-// in order. Items are taken from the last rows (the longest runs of positions) on, in
-// alternating direction, so the CTAs end together.
+// in TMEM; K and V tiles of 128 positions (64 of an f32 cache) feed both. Where the items
+// leave half of the CTAs idle, the positions of each are split evenly and chunk_join_kernel
+// adds the parts in order; a part has one tile at least (8 short prompts in 18.5 us, with
+// empty parts 20.6 us; parts of two tiles or more: 14 prompts over 500 positions in 23.7 us
+// instead of 20.6 us). Items are taken from the last rows (the longest runs of positions)
+// on, in alternating direction, so the CTAs end together: 8,192 rows in 264 us. Equal shares
+// of one line of tiles, as the token kernel has, cost more in items begun twice than they
+// even out (314 us; 240 items of a mixed batch in 126 us instead of 99 us).
 //
 // Roles (one CTA per SM):
 //   warps 0-3, 4-7   softmax of block 0, 1: a thread owns a row, keeps its scores in
@@ -88,7 +92,8 @@ constexpr int kChunkMaxCtas = 160;
 constexpr unsigned long long kWaitNs = 2000000000ull;
 
 constexpr int kChunkMaxParts = kChunkMaxCtas;  // parts of split items in one call: no more than CTAs
-// Workspace of split items: [tile and head] (first row, tokens, kv head, parts), [part] (maximum,
+// Workspace of split items: [tile and head] (first row, tokens, kv head,
+// slots << 16 | parts), [part] (maximum,
 // sum) of 256 rows, numerators [part][256][D].
 __host__ __device__ inline int4* chunk_rec(void* p) { return static_cast<int4*>(p); }
 __host__ __device__ inline float2* chunk_ml(void* p) {
@@ -210,7 +215,7 @@ struct ItemRange {
   int seq, q0, n, len, head, tok0, toks;  // sequence, its first row, new rows, positions; kv head, first token, tokens
   int first;                              // first position of the first tile
   int tiles;                              // tiles of this part
-  int part;                               // partial slot, or -1: the item is whole
+  int part, parts;                        // partial slot, or -1: the item is whole; the item's parts
 };
 
 // token of packed row r (< 128) of a block: r / group
@@ -277,10 +282,16 @@ QORA_DEV ItemRange item_at(const AttnArgs& a, const ItemMap& m, int tokens, int 
   const int hi = min(r.len, p0 + r.toks);           // positions [lo, hi) are attended to
   const int lo = a.window > 0 ? max(0, p0 + 1 - a.window) : 0;
   const int t0 = lo / kPos, nt = max(0, (hi + kPos - 1) / kPos - t0);
-  const int b = (int)(split * (unsigned)nt / (unsigned)splits), e = (int)((split + 1) * (unsigned)nt / (unsigned)splits);
+  r.parts = max(1, min(splits, nt));
+  if (split >= (unsigned)r.parts) {  // a turn that the item has no use for
+    r.toks = r.tiles = 0;
+    r.part = -1;
+    return r;
+  }
+  const int b = (int)((long long)split * nt / r.parts), e = (int)((long long)(split + 1) * nt / r.parts);
   r.first = (t0 + b) * kPos;
   r.tiles = e - b;
-  r.part = splits > 1 ? idx : -1;
+  r.part = r.parts > 1 ? idx : -1;
   return r;
 }
 
@@ -720,8 +731,8 @@ __global__ void __launch_bounds__(ChunkCfg<T, C, D>::kThreads, 1)
       const int seen_from = a.window > 0 ? max(0, p0 + toks - a.window) : 0;
       const bool busy = toks > 0 && it.tiles > 0;
       const long long row0 = it.q0 + it.tok0 + x * block_toks;  // the block's first row
-      if (it.part >= 0 && idx % splits == 0 && tid == 0)
-        chunk_rec(work)[idx / splits] = make_int4((int)row0, it.toks, it.head, splits);
+      if (splits > 1 && idx % splits == 0 && tid == 0)
+        chunk_rec(work)[idx / splits] = make_int4((int)row0, it.parts > 1 ? it.toks : 0, it.head, splits << 16 | it.parts);
       float c = scale2;
       if constexpr (kHalves) {
         // the warp's rows of q, eight at a time: four lanes a row, every fourth float4 each.
@@ -1052,12 +1063,12 @@ template <typename T, int D>
 __global__ void __launch_bounds__(256) chunk_join_kernel(const AttnArgs a, void* work) {
   constexpr int E = D / 32, kAhead = 8;
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int4 rec = chunk_rec(work)[blockIdx.x];  // (first row, tokens, kv head, parts)
-  const int splits = rec.w;
+  const int4 rec = chunk_rec(work)[blockIdx.x];  // (first row, tokens, kv head, slots and parts)
+  const int splits = rec.w & 0xffff;
   const int lane = threadIdx.x & 31, rr = blockIdx.y * 8 + (threadIdx.x >> 5), x = rr >> 7, r = rr & 127;
   const int block_toks = 128 / a.group, rtok = row_token(a, r), tok = x * block_toks + rtok;
   if (rtok >= block_toks || tok >= rec.y) return;
-  const size_t first = (size_t)blockIdx.x * splits * 256 + rr;
+  const size_t first = (size_t)blockIdx.x * (rec.w >> 16) * 256 + rr;
   float mm = -INFINITY;
   for (int s = lane; s < splits; s += 32) mm = fmaxf(mm, chunk_ml(work)[first + (size_t)s * 256].x);
   mm = warp_max(mm);
