@@ -24,6 +24,7 @@ struct AttnArgs {
   int group_inv;      // ceil(2^16 / group)
   int window;         // 0: none
   int max_q;          // no sequence has more new rows
+  int few;            // new rows up to which a sequence is the token kernel's, not the chunk kernel's
   float scale;
   unsigned* status;
 };

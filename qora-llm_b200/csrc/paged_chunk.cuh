@@ -92,6 +92,7 @@ constexpr int kChunkMaxCtas = 160;
 constexpr unsigned long long kWaitNs = 2000000000ull;
 
 constexpr int kChunkMaxParts = kChunkMaxCtas;  // parts of split items in one call: no more than CTAs
+constexpr int kChunkMaxSplit = kChunkMaxCtas / 2;  // split items, of two turns at least
 // Workspace of split items: [tile and head] (first row, tokens, kv head,
 // slots << 16 | parts), [part] (maximum,
 // sum) of 256 rows, numerators [part][256][D].
@@ -232,7 +233,7 @@ QORA_DEV int seq_tiles(const AttnArgs& a, int s, int tokens) {
     if (a.status) *a.status = 5u;
     return 0;
   }
-  return (q1 - q0 + tokens - 1) / tokens;
+  return q1 - q0 <= a.few ? 0 : (q1 - q0 + tokens - 1) / tokens;
 }
 QORA_DEV ItemMap item_map(const AttnArgs& a, int tokens, int lane) {
   ItemMap m;
@@ -410,7 +411,8 @@ __global__ void __launch_bounds__(ChunkCfg<T, C, D>::kThreads, 1)
   const int whole = too_many ? 0 : map.total * a.hk;
   const int splits = split && whole ? max(1, ctas / whole) : 1, items = whole * splits;
   if (split && cta == 0) {  // no rows for the join where there is nothing to join
-    for (int i = (splits > 1 ? whole : 0) + tid; i < max_tiles; i += Cfg::kThreads) chunk_rec(work)[i] = make_int4(0, 0, 0, 0);
+    for (int i = (splits > 1 ? whole : 0) + tid; i < min(max_tiles, kChunkMaxSplit); i += Cfg::kThreads)
+      chunk_rec(work)[i] = make_int4(0, 0, 0, 0);
   }
   // item of turn w: alternating direction, so that long and short items pair up
   auto item_of = [&](int w) { return w * ctas + (w & 1 ? ctas - 1 - cta : cta); };

@@ -144,7 +144,7 @@ qora_status launch_token(const paged::AttnArgs& a, void* work, cudaStream_t s) {
   paged::token_kernel<T, C, D><<<ctas, 32 * Cfg::kWarps, Cfg::kSmem, s>>>(a, work, kTokenMinSteps, kTokenTileCost);
   QCUDA(cudaGetLastError());
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(ctas, std::min<long long>(Cfg::kRows, (long long)a.max_q * a.group));
+  cfg.gridDim = dim3(ctas, std::min(a.max_q, a.few) * a.group);
   cfg.blockDim = dim3(128);
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
@@ -193,13 +193,14 @@ qora_status launch_chunk(const paged::AttnArgs& a, void* work, cudaStream_t s) {
   const int sms = std::min(sm_count(dev), paged::kChunkMaxCtas);
   const int block_toks = Cfg::kBlock / a.group, tokens = 2 * block_toks;
   // Row tiles that sequences with disjoint rows can have, and that they are likely to have
-  // (a half one behind each sequence). Where those leave half of the SMs idle, the kernel
+  // (a half one behind each sequence). Where these leave half of the SMs idle, the kernel
   // splits the items by the number that there are (7 prompts of 45 to 181 rows over up to
   // 2,684 f32 positions: 74.5 us, split by the number that there can be 116 us).
   const long long most = ((long long)a.batch.rows + (long long)a.batch.seqs * (tokens - 1)) / tokens * a.hk;
-  const long long likely = ((long long)a.batch.rows + (long long)a.batch.seqs * (tokens / 2)) / tokens * a.hk;
+  const int long_ones = a.few ? (a.batch.rows + a.max_q - 1) / a.max_q : a.batch.seqs;
+  const long long likely = ((long long)a.batch.rows + (long long)long_ones * (tokens / 2)) / tokens * a.hk;
   if (most > 0x7fffffff) return fail(QORA_ERR_INVALID, "%d rows of %d sequences", a.batch.rows, a.batch.seqs);
-  const bool split = 2 * likely <= sms && most <= paged::kChunkMaxParts;
+  const bool split = 2 * likely <= sms;
   const int ctas = split ? sms : (int)std::min<long long>(sms, most);
   CUtensorMap qmap{}, kmap{}, vmap{};
   int box_rows = 0;
@@ -220,7 +221,7 @@ qora_status launch_chunk(const paged::AttnArgs& a, void* work, cudaStream_t s) {
   QCUDA(cudaGetLastError());
   if (!split) return QORA_OK;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)most, a.max_q > block_toks ? 32 : 16);
+  cfg.gridDim = dim3((unsigned)std::min<long long>(most, paged::kChunkMaxSplit), a.max_q > block_toks ? 32 : 16);
   cfg.blockDim = dim3(256);
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
@@ -232,9 +233,27 @@ qora_status launch_chunk(const paged::AttnArgs& a, void* work, cudaStream_t s) {
   return QORA_OK;
 }
 
+// Sequences with at most `few` new rows are the token kernel's, which reads their pages as
+// fast as memory gives them (64 sequences of 1 to 4 rows over 4,000 positions: 94 us with
+// f16, 184 us with f32 caches; the chunk kernel: 147 us and 540 us for 1 to 5 rows); longer
+// ones the chunk kernel's. Both run where short sequences are likely (the longest is far
+// longer than the mean, or the others are short on average; the host does not know) and
+// are more than the chunk kernel would have in one turn of its CTAs, half of that with an
+// f32 cache: 60 tokens over 4,000 positions with 4 chunks of 512 rows over 2,000 take 147 us
+// with f16, 371 us with f32 caches (the chunk kernel alone: 196 and 711 us), but 31 tokens
+// over 2,000 with a chunk of 256 rows 60 us with f16 caches (alone: 44 us; f32: 98 and 141
+// us). A token kernel without work costs 4 to 10 us.
 template <typename T, typename C, int D>
-qora_status launch_attn(const paged::AttnArgs& a, void* work, cudaStream_t s) {
-  if ((long long)a.max_q * a.group <= paged::TokenCfg<T, C, D>::kRows) return launch_token<T, C, D>(a, work, s);
+qora_status launch_attn(paged::AttnArgs a, void* work, cudaStream_t s) {
+  a.few = paged::TokenCfg<T, C, D>::kRows / a.group;
+  if (a.max_q <= a.few) return launch_token<T, C, D>(a, work, s);
+  const long long rows = a.batch.rows, others = a.batch.seqs - 1;
+  int dev = 0;
+  QCUDA(cudaGetDevice(&dev));
+  const bool many = (others + 1) * a.hk * (sizeof(C) == 4 ? 2 : 1) > sm_count(dev);
+  const bool uneven = 2 * rows <= (others + 1) * a.max_q || rows - a.max_q <= others * a.few;
+  if (!many || !uneven) a.few = 0;
+  if (a.few) QCHECK((launch_token<T, C, D>(a, work, s)));
   return launch_chunk<T, C, D>(a, work, s);
 }
 

@@ -171,7 +171,7 @@ QORA_DEV SeqWork seq_work(const AttnArgs& a, int s) {
     if (a.status) *a.status = 5u;
     return w;
   }
-  if (w.n == 0) return w;
+  if (w.n == 0 || w.n > a.few) return w;
   const int lo = a.window > 0 ? max(0, w.len - w.n + 1 - a.window) : 0;
   w.first = lo & ~(kPos - 1);
   w.steps = max(1, (w.len - w.first + kPos - 1) / kPos);

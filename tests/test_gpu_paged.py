@@ -534,6 +534,24 @@ def test_attention_overlapping_row_ranges_stay_in_bounds(pkg, torch, t, kv):
     assert st == RANGE and np.all(got == -7.0) and np.all(gl == -7.0)
 
 
+@pytest.mark.parametrize("t,kv", TYPES)
+@pytest.mark.parametrize("new,window", [([1] * 40 + [300, 150], 0), ([1, 2, 0, 70, 1, 3, 500, 2] * 5, 200), ([2, 400], 0),
+                                        ([5, 1, 4, 3, 2] * 9, 0), ([700] + [0] * 60 + [1], 0)])
+def test_attention_single_tokens_and_chunks_together(pkg, torch, t, kv, new, window):
+    """One call with single tokens, short runs and long chunks, in any order."""
+    rng = np.random.default_rng(len(new))
+    total = [n + int(rng.integers(0, 1200)) for n in new]
+    b = ref.Batch(rng, new, total, 16)
+    g = torch.Generator(device="cuda").manual_seed(3)
+    pool = Pool(torch, kv, b, 4, 64, "slot")
+    for z in pool.t:
+        z.copy_(torch.randn(z.shape, generator=g, device="cuda"))
+    q = ref.round_to(rng.standard_normal((b.rows, 8, 64)) * 1.5, t)
+    got, gl, st = attend(pkg, torch, b, q, pool, t, window=window)
+    assert st == 0
+    check_on_gpu(torch, b, got, gl, q, pool, t, kv, window)
+
+
 def test_attention_page_offsets_past_32_bits(pkg, torch):
     """A pool of more than 2^32 bytes (and elements past 2^31): pages at its far end."""
     page, hk, d, pages = 64, 4, 128, 70000
