@@ -366,7 +366,8 @@ qora_status qora_q4_lm_head(const float* d_x, const uint8_t* d_packed,
  * [rope_rows][rope_half_dim] f32, both or neither; elements d and d + rope_half_dim turn
  * together, elements from 2 * rope_half_dim on stay (rope_half_dim: a multiple of 8, at most
  * head_dim / 2). d_pos: [rows]; a row with a negative position is padding and stays as it
- * was. q_heads or kv_heads may be 0. Outputs may be the inputs themselves (equal strides). */
+ * was. q_heads or kv_heads may be 0. Outputs may be the inputs themselves (equal strides);
+ * another overlap of rows is refused, here and below. */
 qora_status qora_qk_norm_rope(const void* d_q, uint64_t q_stride, const void* d_k, uint64_t k_stride,
                               uint32_t dtype, uint32_t rows, uint32_t q_heads, uint32_t kv_heads,
                               uint32_t head_dim, const float* d_q_gamma, const float* d_k_gamma,
@@ -398,7 +399,7 @@ qora_status qora_paged_append(const void* d_q, uint64_t q_stride, const void* d_
  * of new rows and for single ones): row i of a sequence attends to positions
  * max(0, p + 1 - window) .. p, p = L - n + i (window 0: from position 0), with weights
  * softmax(scale * q . k); query head h reads kv head h / (q_heads / kv_heads). A row that
- * attends to nothing gets zeros. What is masked does not count, whatever it holds (stale
+ * attends to nothing gets zeros. d_out is another buffer than d_q. What is masked does not count, whatever it holds (stale
  * slots may hold infinities or NaN). d_lse (NULL: not written), [rows][q_heads] f32,
  * receives log(sum exp(scale * q . k)), -inf for a row that attends to nothing. max_q: no
  * sequence has more than max_q new rows (a longer one is out of range). scale > 0.

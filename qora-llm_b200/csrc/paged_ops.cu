@@ -47,9 +47,35 @@ qora_status check_rows(const char* what, const void* p, uint32_t rows, uint64_t 
   return QORA_OK;
 }
 
-qora_status check_same(const char* what, const void* in, uint64_t in_stride, const void* out, uint64_t out_stride) {
-  if (in == out && in_stride != out_stride)
-    return fail(QORA_ERR_INVALID, "%s in place needs equal strides (%llu, %llu)", what, (ull)in_stride, (ull)out_stride);
+// Rows of `width` elements, `stride` apart: what an entry point reads or writes.
+struct Rows {
+  const void* p;
+  uint64_t stride, width;
+};
+// Whether two sets of rows share a byte; those with unequal strides whose ranges meet count
+// as sharing one.
+bool meet(const Rows& a, const Rows& b, uint32_t rows, size_t esz) {
+  const uintptr_t x = (uintptr_t)a.p, y = (uintptr_t)b.p;
+  if (rows == 0 || x + ((rows - 1) * a.stride + a.width) * esz <= y || y + ((rows - 1) * b.stride + b.width) * esz <= x) return false;
+  if (a.stride != b.stride) return true;
+  const uint64_t step = a.stride * esz, off = x <= y ? (y - x) % step : (step - (x - y) % step) % step;  // b's row behind a's
+  return off < a.width * esz || off + b.width * esz > step;
+}
+qora_status check_apart(const char* what, const Rows& a, const Rows& b, uint32_t rows, size_t esz) {
+  if (meet(a, b, rows, esz)) return fail(QORA_ERR_INVALID, "%s overlap", what);
+  return QORA_OK;
+}
+
+qora_status check_same(const char* what, const Rows& in, const Rows& out, uint32_t rows, size_t esz) {
+  if (in.p == out.p && in.stride != out.stride)
+    return fail(QORA_ERR_INVALID, "%s in place needs equal strides (%llu, %llu)", what, (ull)in.stride, (ull)out.stride);
+  if (in.p != out.p && meet(in, out, rows, esz)) return fail(QORA_ERR_INVALID, "%s and its output overlap", what);
+  return QORA_OK;
+}
+
+// Arrays of 32-bit words on the device
+qora_status check_words(const char* what, const void* p) {
+  if ((uintptr_t)p % 4) return fail(QORA_ERR_INVALID, "%s must be 4-byte aligned", what);
   return QORA_OK;
 }
 
@@ -88,6 +114,7 @@ qora_status check_pages(const void* k, const void* v, uint32_t hk, uint32_t head
 qora_status check_batch(const int32_t* q_start, const int32_t* kv_len, const int32_t* table, uint32_t table_stride,
                         uint32_t page_size, uint32_t seqs) {
   if (seqs && (!q_start || !kv_len || !table)) return fail(QORA_ERR_INVALID, "NULL batch arrays");
+  QCHECK(check_words("batch arrays", (const void*)((uintptr_t)q_start | (uintptr_t)kv_len | (uintptr_t)table)));
   if (seqs > (1u << 20)) return fail(QORA_ERR_INVALID, "%u sequences", seqs);
   if (table_stride == 0 || (uint64_t)table_stride * page_size > 0x7fffffffull)
     return fail(QORA_ERR_INVALID, "table rows of %u pages of %u positions", table_stride, page_size);
@@ -279,16 +306,24 @@ qora_status qora_qk_norm_rope(const void* d_q, uint64_t q_stride, const void* d_
   if (q_heads) {
     QCHECK(check_rows("q", d_q, rows, q_stride, q_heads, head_dim, esz));
     QCHECK(check_rows("q_out", d_q_out, rows, q_out_stride, q_heads, head_dim, esz));
-    QCHECK(check_same("q", d_q, q_stride, d_q_out, q_out_stride));
   }
   if (kv_heads) {
     QCHECK(check_rows("k", d_k, rows, k_stride, kv_heads, head_dim, esz));
     QCHECK(check_rows("k_out", d_k_out, rows, k_out_stride, kv_heads, head_dim, esz));
-    QCHECK(check_same("k", d_k, k_stride, d_k_out, k_out_stride));
   }
+  QCHECK(check_words("positions and status", (const void*)((uintptr_t)d_pos | (uintptr_t)d_status)));
   QCHECK(check_turn(d_q_gamma, d_k_gamma, eps, d_cos, d_sin, rope_rows, rope_half_dim, head_dim));
   if (d_cos && !d_pos && rows) return fail(QORA_ERR_INVALID, "a rotation needs positions");
   if (rows == 0) return QORA_OK;
+  const Rows q{d_q, q_stride, (uint64_t)q_heads * head_dim}, qo{d_q_out, q_out_stride, q.width};
+  const Rows k{d_k, k_stride, (uint64_t)kv_heads * head_dim}, ko{d_k_out, k_out_stride, k.width};
+  if (q_heads) QCHECK(check_same("q", q, qo, rows, esz));
+  if (kv_heads) QCHECK(check_same("k", k, ko, rows, esz));
+  if (q_heads && kv_heads) {
+    QCHECK(check_apart("q_out and k", qo, k, rows, esz));
+    QCHECK(check_apart("k_out and q", ko, q, rows, esz));
+    QCHECK(check_apart("q_out and k_out", qo, ko, rows, esz));
+  }
   paged::RowArgs a{};
   a.q = d_q, a.k = d_k, a.q_stride = (long long)q_stride, a.k_stride = (long long)k_stride;
   a.rows = (int)rows, a.hq = (int)q_heads, a.hk = (int)kv_heads, a.hv = 0;
@@ -319,15 +354,21 @@ qora_status qora_paged_append(const void* d_q, uint64_t q_stride, const void* d_
   if (q_heads) {
     QCHECK(check_rows("q", d_q, rows, q_stride, q_heads, head_dim, esz));
     QCHECK(check_rows("q_out", d_q_out, rows, q_out_stride, q_heads, head_dim, esz));
-    QCHECK(check_same("q", d_q, q_stride, d_q_out, q_out_stride));
   }
   QCHECK(check_rows("k", d_k, rows, k_stride, kv_heads, head_dim, esz));
   QCHECK(check_rows("v", d_v, rows, v_stride, kv_heads, head_dim, esz));
+  QCHECK(check_words("status", d_status));
   QCHECK(check_turn(d_q_gamma, d_k_gamma, eps, d_cos, d_sin, rope_rows, rope_half_dim, head_dim));
   QCHECK(check_pages(d_k_pages, d_v_pages, kv_heads, head_dim, elem_size(kv_dtype), num_pages, page_size, page_stride,
                      head_stride, slot_stride));
   QCHECK(check_batch(d_q_start, d_kv_len, d_table, table_stride, page_size, seqs));
   if (rows == 0 || seqs == 0) return QORA_OK;
+  if (q_heads) {
+    const Rows q{d_q, q_stride, (uint64_t)q_heads * head_dim}, qo{d_q_out, q_out_stride, q.width};
+    QCHECK(check_same("q", q, qo, rows, esz));
+    QCHECK(check_apart("q_out and k", qo, {d_k, k_stride, (uint64_t)kv_heads * head_dim}, rows, esz));
+    QCHECK(check_apart("q_out and v", qo, {d_v, v_stride, (uint64_t)kv_heads * head_dim}, rows, esz));
+  }
   paged::RowArgs a{};
   a.q = d_q, a.k = d_k, a.v = d_v;
   a.q_stride = (long long)q_stride, a.k_stride = (long long)k_stride, a.v_stride = (long long)v_stride;
@@ -361,6 +402,7 @@ qora_status qora_paged_attention(const void* d_q, uint64_t q_stride, uint32_t dt
   const size_t esz = elem_size(dtype);
   QCHECK(check_rows("q", d_q, rows, q_stride, q_heads, head_dim, esz));
   QCHECK(check_rows("out", d_out, rows, out_stride, q_heads, head_dim, esz));
+  QCHECK(check_words("lse and status", (const void*)((uintptr_t)d_lse | (uintptr_t)d_status)));
   if (!(scale > 0.0f) || !std::isfinite(2.0f * scale)) return fail(QORA_ERR_INVALID, "scale %g", (double)scale);
   if (window > 0x7fffffffu) return fail(QORA_ERR_INVALID, "window %u", window);
   QCHECK(check_pages(d_k_pages, d_v_pages, kv_heads, head_dim, elem_size(kv_dtype), num_pages, page_size, page_stride,
@@ -370,6 +412,7 @@ qora_status qora_paged_attention(const void* d_q, uint64_t q_stride, uint32_t dt
     return fail(QORA_ERR_INVALID, "the workspace needs %u bytes on a 256-byte boundary", QORA_PAGED_WORK_BYTES);
   if (rows == 0 || seqs == 0) return QORA_OK;
   if (max_q == 0) return fail(QORA_ERR_INVALID, "max_q is 0");
+  QCHECK(check_apart("q and out", {d_q, q_stride, (uint64_t)q_heads * head_dim}, {d_out, out_stride, (uint64_t)q_heads * head_dim}, rows, esz));
   paged::AttnArgs a{};
   a.q = d_q, a.q_stride = (long long)q_stride;
   a.out = d_out, a.out_stride = (long long)out_stride;

@@ -115,6 +115,47 @@ def test_empty_arrays_may_be_null(pkg):
     pkg.engine.paged_attention(**attend_args(rows=0, seqs=0, max_q=0, q_ptr=None, out_ptr=None, kv_len_ptr=None, table_ptr=None))
 
 
+M = 1 << 16  # bytes beyond the rows of the calls above
+
+
+@pytest.mark.parametrize("fn,args,match", [
+    ("qk_norm_rope", norm_args(q_out_ptr=A + 64, k_ptr=A + M, k_out_ptr=A + M), "q and its output"),
+    ("qk_norm_rope", norm_args(k_ptr=A + M, k_out_ptr=A + M + 512), "k and its output"),
+    ("qk_norm_rope", norm_args(k_ptr=A + 1024, k_out_ptr=A + M), "q_out and k overlap"),
+    ("qk_norm_rope", norm_args(k_ptr=A + M, k_out_ptr=A + 4096, q_ptr=A, q_out_ptr=A + 2 * M), "k_out and q"),
+    ("qk_norm_rope", norm_args(k_ptr=A + M, k_out_ptr=A + 2 * M, q_out_ptr=A + 2 * M), "q_out and k_out"),
+    ("paged_append", append_args(q_heads=8, q_ptr=A + M, q_out_ptr=A + M + 16), "q and its output"),
+    ("paged_append", append_args(q_heads=8, q_ptr=A + M, q_out_ptr=A, v_ptr=A + 2 * M), "q_out and k"),
+    ("paged_append", append_args(q_heads=8, q_ptr=A + M, q_out_ptr=A, k_ptr=A + 2 * M), "q_out and v"),
+    ("paged_attention", attend_args(), "q and out"), ("paged_attention", attend_args(out_ptr=A + 2 * 4096), "q and out"),
+])
+def test_overlapping_rows_are_refused(pkg, fn, args, match):
+    refused(pkg, getattr(pkg.engine, fn), args, INVALID, match)
+
+
+def test_parts_of_one_joined_row_do_not_overlap(pkg):
+    """Accepted as far as the rows go: what refuses these calls is the last check."""
+    w = (8 + 2 + 2) * 128
+    joined = dict(q_stride=w, k_stride=w, dtype="f32")
+    with pytest.raises(pkg.QoraError, match="go together"):
+        pkg.engine.qk_norm_rope(**norm_args(**joined, k_ptr=A + 4096, k_out_ptr=A + 4096, q_out_stride=w, k_out_stride=w, sin_ptr=None))
+    with pytest.raises(pkg.QoraError, match="pages of 0"):
+        pkg.engine.paged_append(**append_args(**joined, q_heads=8, q_ptr=A, q_out_ptr=A, q_out_stride=w, k_ptr=A + 4096,
+                                              v_ptr=A + 4096 + 1024, v_stride=w, page_size=0))
+    with pytest.raises(pkg.QoraError, match="scale"):
+        pkg.engine.paged_attention(**attend_args(q_stride=2048, out_ptr=A + 4096, out_stride=2048, scale=0.0))
+
+
+@pytest.mark.parametrize("fn,args,match", [
+    ("qk_norm_rope", norm_args(k_ptr=A + M, k_out_ptr=A + M, pos_ptr=A + 2), "4-byte"),
+    ("paged_append", append_args(kv_len_ptr=A + 1), "4-byte"), ("paged_append", append_args(status_ptr=A + 2), "4-byte"),
+    ("paged_attention", attend_args(out_ptr=A + M, lse_ptr=A + 2), "4-byte"),
+    ("paged_attention", attend_args(out_ptr=A + M, table_ptr=A + 3), "4-byte"),
+])
+def test_misaligned_words_are_refused(pkg, fn, args, match):
+    refused(pkg, getattr(pkg.engine, fn), args, INVALID, match)
+
+
 def test_scale_that_leaves_f32(pkg):
     refused(pkg, pkg.engine.paged_attention, attend_args(scale=3e38), INVALID, "scale")
 
