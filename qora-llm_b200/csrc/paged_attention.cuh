@@ -29,5 +29,9 @@ struct AttnArgs {
   unsigned* status;
 };
 
+// The first position that a row at position p attends to. p may be negative (more new rows
+// than positions), the window up to 2^31 - 1.
+QORA_DEV int first_seen(const AttnArgs& a, int p) { return a.window > 0 ? max(0, max(p, -1) + 1 - a.window) : 0; }
+
 }  // namespace paged
 }  // namespace qora

@@ -285,7 +285,7 @@ QORA_DEV ItemRange item_at(const AttnArgs& a, const ItemMap& m, int tokens, int 
   r.toks = min(tokens, r.n - r.tok0);
   const int p0 = r.len - r.n + r.tok0;              // position of the first row
   const int hi = min(r.len, p0 + r.toks);           // positions [lo, hi) are attended to
-  const int lo = a.window > 0 ? max(0, p0 + 1 - a.window) : 0;
+  const int lo = first_seen(a, p0);
   const int t0 = lo / kPos, nt = max(0, (hi + kPos - 1) / kPos - t0);
   r.parts = max(1, min(splits, nt));
   if (split >= (unsigned)r.parts) {  // a turn that the item has no use for
@@ -732,9 +732,9 @@ __global__ void __launch_bounds__(ChunkCfg<T, C, D>::kThreads, 1)
       const bool live = rtok < toks;
       const int p0 = it.len - it.n + it.tok0 + x * block_toks;  // position of the block's first token
       const int plast = live ? p0 + rtok : -1;
-      const int pfirst = a.window > 0 ? max(0, plast + 1 - a.window) : 0;
+      const int pfirst = first_seen(a, plast);
       // every row of the block sees the positions from seen_from to p0
-      const int seen_from = a.window > 0 ? max(0, p0 + toks - a.window) : 0;
+      const int seen_from = first_seen(a, p0 + toks - 1);
       const bool busy = toks > 0 && it.tiles > 0;
       const long long row0 = it.q0 + it.tok0 + x * block_toks;  // the block's first row
       if (splits > 1 && idx % splits == 0 && tid == 0)

@@ -172,7 +172,7 @@ QORA_DEV SeqWork seq_work(const AttnArgs& a, int s) {
     return w;
   }
   if (w.n == 0 || w.n > a.few) return w;
-  const int lo = a.window > 0 ? max(0, w.len - w.n + 1 - a.window) : 0;
+  const int lo = first_seen(a, w.len - w.n);
   w.first = lo & ~(kPos - 1);
   w.steps = max(1, (w.len - w.first + kPos - 1) / kPos);
   return w;
@@ -290,10 +290,10 @@ __global__ void __launch_bounds__(32 * TokenCfg<T, C, D>::kWarps, 1) token_kerne
       const int r = g + 8 * i;
       const bool ok = (!kHalves || i == 0) && r < nrows;
       plast[i] = ok ? p0 + token_of(a, r) : -1;
-      pfirst[i] = a.window > 0 ? max(0, plast[i] + 1 - a.window) : 0;
+      pfirst[i] = first_seen(a, plast[i]);
     }
     // every row sees the positions from seen_from to p0
-    const int seen_from = a.window > 0 ? max(0, sw.len - a.window) : 0;
+    const int seen_from = first_seen(a, sw.len - 1);
 
     // offset of position `pos` in the pages; -1: nothing there
     auto page_of = [&](int pos) -> int {
