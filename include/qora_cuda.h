@@ -340,7 +340,9 @@ qora_status qora_q4_lm_head(const float* d_x, const uint8_t* d_packed,
  * slot p % page_size; element (page, head, slot, d) of the K (V) pages is at d_k_pages
  * (d_v_pages) + page * page_stride + head * head_stride + slot * slot_stride + d (elements,
  * multiples of 16 bytes). [page][slot][head][d] and [page][head][slot][d] are both taken,
- * with any page_size. Table entries past a sequence's last position are not read.
+ * with any page_size. Table entries past a sequence's last position, and for an attention
+ * with a window those before the first position that its new rows attend to (released
+ * pages), need not name a page.
  *
  * Types. Rows f32 with pages f32 or f16, rows and pages f16, rows and pages bf16. Sums,
  * norms and softmax statistics are f32 throughout; a value is rounded once, to nearest

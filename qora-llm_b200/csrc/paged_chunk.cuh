@@ -218,7 +218,7 @@ __host__ __device__ constexpr uint32_t chunk_idesc(int n, bool b_mn) {
 // ---------------------------------------------------------------- items
 struct ItemRange {
   int seq, q0, n, len, head, tok0, toks;  // sequence, its first row, new rows, positions; kv head, first token, tokens
-  int first;                              // first position of the first tile
+  int lo, first;                          // first attended position, first position of the first tile
   int tiles;                              // tiles of this part
   int part, parts;                        // partial slot, or -1: the item is whole; the item's parts
 };
@@ -286,6 +286,7 @@ QORA_DEV ItemRange item_at(const AttnArgs& a, const ItemMap& m, int tokens, int 
   const int p0 = r.len - r.n + r.tok0;              // position of the first row
   const int hi = min(r.len, p0 + r.toks);           // positions [lo, hi) are attended to
   const int lo = first_seen(a, p0);
+  r.lo = lo;
   const int t0 = lo / kPos, nt = max(0, (hi + kPos - 1) / kPos - t0);
   r.parts = max(1, min(splits, nt));
   if (split >= (unsigned)r.parts) {  // a turn that the item has no use for
@@ -579,7 +580,9 @@ __global__ void __launch_bounds__(ChunkCfg<T, C, D>::kThreads, 1)
       const int* table = a.batch.table + (long long)it.seq * a.batch.table_stride;
       const C* base = static_cast<const C*>(team ? a.v_pages : a.k_pages) + it.head * a.pg.head_stride;
       const C* vbase = static_cast<const C*>(a.v_pages) + it.head * a.pg.head_stride;
-      // a tile's boxes: lane i holds the page of box i, looked up a tile ahead
+      // a tile's boxes: lane i holds the page of box i, looked up a tile ahead. Entries before
+      // the first attended position may be those of released pages: where they name no page,
+      // the tile is copied by position, and they are not looked at
       const int boxes = box_rows ? kPos / box_rows : 0;
       auto box_page = [&](int j) {
         const int pos = it.first + j * kPos + lane * box_rows;
@@ -623,7 +626,7 @@ __global__ void __launch_bounds__(ChunkCfg<T, C, D>::kThreads, 1)
         for (int i = lt; i < kPos; i += kLoaders) {
           const int pos = tile0 + i;
           long long off = -1;
-          if (pos < it.len) {
+          if (pos >= it.lo && pos < it.len) {
             const int page = table[pos / a.pg.page_size];
             if (page >= 0 && page < a.pg.num_pages)
               off = page * a.pg.page_stride + (long long)(pos % a.pg.page_size) * a.pg.slot_stride;

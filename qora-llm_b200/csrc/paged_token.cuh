@@ -155,7 +155,7 @@ __host__ __device__ inline TokenWork token_work(void* p, int ctas) {
 
 // One sequence's share of the line of steps: hk tiles of `steps` steps.
 struct SeqWork {
-  int q0, n, len, first;  // first row, new rows, positions, first step's position
+  int q0, n, len, lo, first;  // first row, new rows, positions, first attended one, first step's
   int steps;
 };
 template <int kPos>
@@ -165,15 +165,15 @@ QORA_DEV SeqWork seq_work(const AttnArgs& a, int s) {
   const int q1 = a.batch.q_start[s + 1];
   w.len = a.batch.kv_len[s];
   w.n = q1 - w.q0;
-  w.first = w.steps = 0;
+  w.lo = w.first = w.steps = 0;
   const long long cap = (long long)a.batch.table_stride * a.pg.page_size;
   if (w.q0 < 0 || q1 < w.q0 || q1 > a.batch.rows || w.n > a.max_q || w.len < 0 || w.len > cap) {
     if (a.status) *a.status = 5u;
     return w;
   }
   if (w.n == 0 || w.n > a.few) return w;
-  const int lo = first_seen(a, w.len - w.n);
-  w.first = lo & ~(kPos - 1);
+  w.lo = first_seen(a, w.len - w.n);
+  w.first = w.lo & ~(kPos - 1);
   w.steps = max(1, (w.len - w.first + kPos - 1) / kPos);
   return w;
 }
@@ -295,9 +295,10 @@ __global__ void __launch_bounds__(32 * TokenCfg<T, C, D>::kWarps, 1) token_kerne
     // every row sees the positions from seen_from to p0
     const int seen_from = first_seen(a, sw.len - 1);
 
-    // offset of position `pos` in the pages; -1: nothing there
+    // offset of position `pos` in the pages; -1: nothing there. Entries before the first
+    // attended position may be those of released pages: not read
     auto page_of = [&](int pos) -> int {
-      if (pos >= sw.len) return -1;
+      if (pos >= sw.len || pos < sw.lo) return -1;
       return table[pow2 ? pos >> shift : pos / a.pg.page_size];
     };
     auto offset_of = [&](int pos, int page) -> long long {
@@ -311,7 +312,8 @@ __global__ void __launch_bounds__(32 * TokenCfg<T, C, D>::kWarps, 1) token_kerne
       const int pos = sw.first + step * kPos;
       const int left = sw.len - pos;  // positions that there are from here on
       const uint32_t dk = ptx::smem_addr(ring + stage * Cfg::kStep), dv = dk + Cfg::kSide;
-      const unsigned gone = left >= kPos ? 0u : ~0u << max(0, left) & ((1u << kPos) - 1);
+      const unsigned ahead = pos < sw.lo ? (1u << (sw.lo - pos)) - 1 : 0u;  // not attended to (first step)
+      const unsigned gone = (left >= kPos ? 0u : ~0u << max(0, left) & ((1u << kPos) - 1)) | ahead;
       const long long off = offset_of(pos + (lane & (kPos - 1)), page);
       const unsigned bad = __ballot_sync(0xffffffffu, off < 0) & ((1u << kPos) - 1);
 #pragma unroll

@@ -2,7 +2,8 @@
 import numpy as np
 import pytest
 
-from test_gpu_paged import TYPES, attend, check_attention, make
+import paged_ref as ref
+from test_gpu_paged import RANGE, TYPES, Pool, attend, check_attention, check_on_gpu, make
 from test_gpu_paged import torch as torch  # the fixture
 
 pytestmark = pytest.mark.gpu
@@ -19,3 +20,48 @@ def test_windows_wider_than_any_sequence(pkg, torch, t, kv, window, new, total):
     got, gl, st = attend(pkg, torch, b, q, pool, t, window=window)
     assert st == 0
     check_attention(b, got, gl, q, pages, t, kv, 0.125, 0)
+
+
+@pytest.mark.parametrize("t,kv", TYPES)
+@pytest.mark.parametrize("page,layout,d", [(1, "slot", 64), (7, "head", 128), (8, "slot", 128), (16, "head", 128), (24, "slot", 64),
+                                           (64, "slot", 128), (128, "head", 64)])
+@pytest.mark.parametrize("new,total,window", [([1, 1, 1], [700, 331, 20], 100), ([3, 2], [515, 260], 33), ([70, 40], [700, 415], 70),
+                                              ([1, 90, 2, 1], [400, 777, 90, 300], 129)])
+def test_pages_released_behind_the_window(pkg, torch, t, kv, page, layout, d, new, total, window):
+    """Table entries before the first position that a sequence's new rows attend to name no page."""
+    rng = np.random.default_rng(page + len(new))
+    b, q, pages, pool = make(torch, rng, t, kv, new, total, page, layout, 4, 2, d)
+    live = b.table.copy()
+    dead = 0
+    for s in range(b.seqs):
+        gone = max(0, total[s] - new[s] + 1 - window) // page
+        b.table[s, :gone] = np.resize([-1, b.pages, 2**31 - 1, -2**31], gone)
+        dead += gone
+    assert dead
+    got, gl, st = attend(pkg, torch, b, q, pool, t, window=window)
+    assert st == 0
+    b.table = live
+    check_attention(b, got, gl, q, pages, t, kv, d ** -0.5, window)
+
+
+@pytest.mark.parametrize("t,kv", TYPES)
+@pytest.mark.parametrize("new", [[1], [2], [300]])
+def test_released_pages_of_long_caches(pkg, torch, t, kv, new):
+    """The same where the work is split over the positions; a bad page that a row does attend to still counts."""
+    g = torch.Generator(device="cuda").manual_seed(1)
+    L, window, page = 6000, 2500, 16
+    b = ref.Batch(np.random.default_rng(2), new, [L], page)
+    pool = Pool(torch, kv, b, 2, 128, "slot")
+    for z in pool.t:
+        z.copy_(torch.randn(z.shape, generator=g, device="cuda"))
+    q = ref.round_to(np.random.default_rng(3).standard_normal((b.rows, 4, 128)), t)
+    live, first = b.table.copy(), max(0, L - new[0] + 1 - window)
+    b.table[0, :first // page] = -1
+    got, gl, st = attend(pkg, torch, b, q, pool, t, window=window)
+    assert st == 0
+    bad = b.table.copy()
+    b.table = live
+    check_on_gpu(torch, b, got, gl, q, pool, t, kv, window)
+    bad[0, first // page] = -1
+    b.table = bad
+    assert attend(pkg, torch, b, q, pool, t, window=window)[2] == RANGE
