@@ -43,13 +43,21 @@ QORA_DEV void tmem_ld8(uint32_t taddr, uint32_t (&v)[8]) {
 }
 QORA_DEV void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
-// bounded mbarrier wait; false (and the CTA's abort flag set) after limit_ns
-QORA_DEV bool wait_bar(uint64_t* bar, uint32_t parity, unsigned long long limit_ns, volatile int* abort) {
+// bounded mbarrier wait; false (and the CTA's abort flag set) after limit_ns. `progress`: a
+// counter in shared memory that warps raise while they do work of unbounded length; the limit
+// counts from its last change
+QORA_DEV bool wait_bar(uint64_t* bar, uint32_t parity, unsigned long long limit_ns, volatile int* abort,
+                       volatile unsigned* progress = nullptr) {
   if (ptx::mbar_try_wait(bar, parity)) return true;
-  const uint64_t t0 = ptx::globaltimer();
+  uint64_t t0 = ptx::globaltimer();
+  unsigned seen = progress ? *progress : 0u;
   for (;;) {
     if (ptx::mbar_try_wait(bar, parity)) return true;
     if (*abort) return false;
+    if (progress && *progress != seen) {
+      seen = *progress;
+      t0 = ptx::globaltimer();
+    }
     if (ptx::globaltimer() - t0 > limit_ns) {
       *abort = 1;
       return false;

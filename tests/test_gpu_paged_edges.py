@@ -65,3 +65,49 @@ def test_released_pages_of_long_caches(pkg, torch, t, kv, new):
     bad[0, first // page] = -1
     b.table = bad
     assert attend(pkg, torch, b, q, pool, t, window=window)[2] == RANGE
+
+
+# ---------------------------------------------------------------- rows that are computed again
+@pytest.mark.parametrize("t,kv", TYPES)
+@pytest.mark.parametrize("new,total,hq,hk", [([1500], [1500], 8, 4), ([300] * 6, [1300 - 70 * s for s in range(6)], 16, 4), ([50], [2900], 8, 2)])
+def test_rows_that_are_computed_again_among_others(pkg, torch, t, kv, new, total, hq, hk):
+    """An infinite value early in one head of each sequence: all of the head's rows are computed
+    again, several items per CTA (and split ones); element 7 is infinite, everything else as ever."""
+    b = ref.Batch(np.random.default_rng(1), new, total, 16)
+    g = torch.Generator(device="cuda").manual_seed(5)
+    pool = Pool(torch, kv, b, hk, 64, "slot")
+    for z in pool.t:
+        z.copy_(torch.randn(z.shape, generator=g, device="cuda"))
+    q = ref.round_to(np.random.default_rng(2).standard_normal((b.rows, hq, 64)) * 1.5, t)
+    at = [b.place(s, 5) for s in range(b.seqs)]
+    for pg, sl in at:
+        pool.t[1][pg, sl, 1, 7] = np.inf
+    got, gl, st = attend(pkg, torch, b, q, pool, t)
+    assert st == 0
+    reach = np.zeros((b.rows, hq), bool)
+    for s in range(b.seqs):
+        for i in range(new[s]):
+            reach[b.start[s] + i, hq // hk:2 * hq // hk] = total[s] - new[s] + i >= 5
+    assert np.isposinf(got[reach][:, 7]).all() and np.isfinite(got[~reach]).all()
+    for pg, sl in at:
+        pool.t[1][pg, sl, 1, 7] = 0.0
+    clean, _, _ = attend(pkg, torch, b, q, pool, t)
+    got[..., 7] = np.where(reach, clean[..., 7], got[..., 7])
+    check_on_gpu(torch, b, got, gl, q, pool, t, kv)
+
+
+@pytest.mark.parametrize("new,total", [([1100], [1100]), ([40], [4500])])
+@pytest.mark.parametrize("which", [0, 1])
+def test_f32_rows_of_unlike_size_in_one_tile(pkg, torch, new, total, which):
+    """A row of K (V) 1e-6 times its neighbours': its tile's rows are computed again."""
+    b = ref.Batch(np.random.default_rng(1), new, total, 16)
+    g = torch.Generator(device="cuda").manual_seed(6)
+    pool = Pool(torch, "f32", b, 2, 128, "head")
+    for z in pool.t:
+        z.copy_(torch.randn(z.shape, generator=g, device="cuda"))
+    pg, sl = b.place(0, 100)
+    pool.t[which][pg, :, sl] *= 1e-6
+    q = ref.round_to(np.random.default_rng(2).standard_normal((b.rows, 4, 128)) * 1.5, "f32")
+    got, gl, st = attend(pkg, torch, b, q, pool, "f32")
+    assert st == 0
+    check_on_gpu(torch, b, got, gl, q, pool, "f32", "f32")
