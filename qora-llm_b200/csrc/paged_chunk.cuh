@@ -503,16 +503,16 @@ __global__ void __launch_bounds__(ChunkCfg<T, C, D>::kThreads, 1)
       ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
       tile += it.tiles;
     }
-    // every product has completed before the TMEM goes
+    // every product has completed before the TMEM and the tiles go
     if (lane == 0) {
       umma::mma_commit(done);
-      umma::wait_bar(done, 0, kWaitNs, abort_flag);
+      umma::settle_bar(done, 0, kWaitNs);
     }
     __syncwarp();
   } else if (!kWide && warp == 11) {
     // -------------------------------------------------------------------- q of 16-bit rows
     if constexpr (!kHalves) {
-      uint32_t turn = 0;
+      uint32_t turn = 0, loads[2] = {0, 0};
       for (int w = 0; w * ctas < items; ++w) {
         const int idx = item_of(w);
         if (idx >= items) continue;
@@ -528,11 +528,16 @@ __global__ void __launch_bounds__(ChunkCfg<T, C, D>::kThreads, 1)
             for (int h = 0; h < D / 64; ++h)
               tma_3d(ptx::smem_addr(sq + x * Cfg::kQTile + h * kHalfQ), &qmap, 64 * h, it.head * a.group,
                      it.q0 + it.tok0 + x * block_toks, q_full + x);
+            ++loads[x];
           }
         }
         __syncwarp();
         ++turn;
       }
+      // every copy has landed before the shared memory goes
+      if (lane == 0)
+        for (int x = 0; x < 2; ++x)
+          if (loads[x]) umma::settle_bar(q_full + x, (loads[x] - 1) & 1, kWaitNs);
     }
   } else if (warp > 8) {
     // -------------------------------------------------------------------- K and V
@@ -543,10 +548,12 @@ __global__ void __launch_bounds__(ChunkCfg<T, C, D>::kThreads, 1)
     bool ok = true, stop = false;  // this thread's waits ended in time; the team's threads agree to stop
     uint64_t* pend[kLag];          // barriers of the copies still in flight
     int np = 0;
-    // one arrival for the team's threads, each of which has fenced its own writes
+    uint32_t copied = 0, odd = 0;  // stages that TMA filled last, and the parity of that phase
+    // one arrival for the team's threads, each of which has fenced its own writes; none on a
+    // stage that did not come free (null)
     auto arrive = [&](uint64_t* bar) {
       ptx::named_bar(bar_id, kLoaders);
-      if (lt == 0) ptx::mbar_arrive(bar);
+      if (lt == 0 && bar) ptx::mbar_arrive(bar);
     };
     auto flush = [&]() {
       asm volatile("cp.async.wait_all;" ::: "memory");
@@ -609,6 +616,11 @@ __global__ void __launch_bounds__(ChunkCfg<T, C, D>::kThreads, 1)
                 ok = ok && __all_sync(0xffffffffu, wait(empty + st, ((entry / kStages) & 1) ^ 1));
                 if (!ok) continue;
                 if (lane == 0) ptx::mbar_arrive_expect_tx(full + st, Cfg::kStage);
+                copied |= 1u << st;
+                if ((entry / kStages) & 1)
+                  odd |= 1u << st;
+                else
+                  odd &= ~(1u << st);
                 __syncwarp();
                 if (lane < boxes) {
                   const int slot = (tile0 + lane * box_rows) % a.pg.page_size;
@@ -660,7 +672,8 @@ __global__ void __launch_bounds__(ChunkCfg<T, C, D>::kThreads, 1)
               const long long o = s_off[r];
               cp_async_16(dst + tile_at(r, pc, kHalfKV), basep + (o < 0 ? 0 : o), o >= 0);
             }
-            landed(full + st);
+            if (free) copied &= ~(1u << st);
+            landed(ok ? full + st : nullptr);
           }
         } else {
           constexpr int kF4 = D / 4;            // float4s of a row
@@ -716,13 +729,17 @@ __global__ void __launch_bounds__(ChunkCfg<T, C, D>::kThreads, 1)
             }
           }
           ptx::fence_proxy_async();
-          arrive(full + st);
+          arrive(ok ? full + st : nullptr);
           entry += 2;
         }
       }
       tiles += it.tiles;
     }
     flush();
+    // every copy has landed before the shared memory goes
+    if (!kWide && lw == 0 && lane == 0)
+      for (int st = 0; st < kStages; ++st)
+        if ((copied >> st) & 1) umma::settle_bar(full + st, (odd >> st) & 1, kWaitNs);
   } else {
     // -------------------------------------------------------------------- softmax
     const int x = warp >> 2, r0 = (warp & 3) * 32, r = r0 + lane;

@@ -65,5 +65,15 @@ QORA_DEV bool wait_bar(uint64_t* bar, uint32_t parity, unsigned long long limit_
   }
 }
 
+// Before the end of a kernel that may have given up: bounded wait for what this thread's copies
+// or products arrive on, whatever the abort flag says (shared memory and TMEM must not be
+// handed on under them)
+QORA_DEV bool settle_bar(uint64_t* bar, uint32_t parity, unsigned long long limit_ns) {
+  const uint64_t t0 = ptx::globaltimer();
+  while (!ptx::mbar_try_wait(bar, parity))
+    if (ptx::globaltimer() - t0 > limit_ns) return false;
+  return true;
+}
+
 }  // namespace umma
 }  // namespace qora

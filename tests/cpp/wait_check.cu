@@ -1,6 +1,7 @@
 // The bounded waits of tcgen05.cuh on a GPU, each with a limit of a few milliseconds: a wait
 // whose partner reports progress outlasts the limit and ends when the barrier completes; one
-// without progress gives up, sets the abort flag and returns. Prints "ok".
+// without progress gives up, sets the abort flag and returns. Settling waits for copies in
+// flight and has a limit too. Prints "ok".
 #include <cstdio>
 
 #include "../../qora-llm_b200/csrc/tcgen05.cuh"
@@ -39,9 +40,32 @@ __global__ void wait_kernel(int rounds, int arrive, int counted, int* out) {
   __syncthreads();
 }
 
+// A bulk copy under way when the CTA has already given up: settling waits for it, so that the
+// data is there; settling on a barrier that nothing arrives on ends at the limit.
+__global__ void settle_kernel(const int* src, int* out) {
+  __shared__ alignas(128) int data[8192];
+  __shared__ uint64_t bars[2];
+  if (threadIdx.x == 0) {
+    ptx::mbar_init(&bars[0], 1);
+    ptx::mbar_init(&bars[1], 1);
+    ptx::fence_mbar_init();
+    data[8191] = -1;
+    ptx::fence_proxy_async();
+    ptx::mbar_arrive_expect_tx(&bars[0], sizeof(data));
+    ptx::bulk_g2s(data, src, sizeof(data), &bars[0]);
+    out[0] = umma::settle_bar(&bars[0], 0, 1000 * kLimit);
+    out[1] = data[8191];
+    const uint64_t t0 = ptx::globaltimer();
+    out[2] = umma::settle_bar(&bars[1], 0, kLimit);
+    out[3] = (int)((ptx::globaltimer() - t0) / 1000);
+  }
+}
+
 int main() {
-  int* out;
-  if (cudaMallocManaged(&out, 3 * sizeof(int)) != cudaSuccess) return std::printf("no device memory\n"), 1;
+  int *out, *src;
+  if (cudaMallocManaged(&out, 4 * sizeof(int)) != cudaSuccess || cudaMalloc(&src, 8192 * sizeof(int)) != cudaSuccess ||
+      cudaMemset(src, 5, 8192 * sizeof(int)) != cudaSuccess)
+    return std::printf("no device memory\n"), 1;
   struct Case {
     int rounds, arrive, counted, ended, least_us;
   };
@@ -56,6 +80,9 @@ int main() {
       return 1;
     }
   }
+  settle_kernel<<<1, 32>>>(src, out);
+  if (cudaDeviceSynchronize() != cudaSuccess || out[0] != 1 || out[1] != 0x05050505 || out[2] != 0 || out[3] < 2900)
+    return std::printf("FAIL settle: %d, data %x; %d, %d us\n", out[0], out[1], out[2], out[3]), 1;
   std::printf("ok\n");
   return 0;
 }
