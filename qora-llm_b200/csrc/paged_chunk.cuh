@@ -1048,6 +1048,7 @@ __global__ void __launch_bounds__(ChunkCfg<T, C, D>::kThreads, 1)
       // rows to compute again, one after the other by the whole warp
       redo &= live_rows;
       if (redo) {
+        __syncwarp();  // other lanes have stored what is stored again here
         const int* table = a.batch.table + (long long)it.seq * a.batch.table_stride;
         for (; redo; redo &= redo - 1) {
           const int src = __ffs(redo) - 1, rr = r0 + src, tok = row_token(a, rr);
