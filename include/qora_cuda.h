@@ -356,7 +356,13 @@ qora_status qora_q4_lm_head(const float* d_x, const uint8_t* d_packed,
  * [0, rows) or whose length does not fit its table row, a position behind the rotation
  * tables, a page id outside [0, num_pages). What is out of range is skipped (its rows stay
  * as they were; positions on a bad page count as masked) and *d_status (NULL: not
- * reported) is set to QORA_ERR_RANGE. The library never clears *d_status.
+ * reported) is set to QORA_ERR_RANGE. So it is where the attention's count of a batch's work
+ * is full: kv heads times (positions + 512 for each sequence) reaches 2^29 (16-bit caches:
+ * 2^30) for one sequence of few new rows, or for seqs / 32 neighbouring ones; no such sequence
+ * of the call is computed. QORA_ERR_TIMEOUT in *d_status says that a wait inside the attention
+ * ran out, which only a fault of the device or of the library brings about, never the size of
+ * the work; the call's rows are then not defined (with a NULL d_status nothing tells). The
+ * library never clears *d_status.
  * ---------------------------------------------------------------------------------- */
 #define QORA_DT_F32  0u
 #define QORA_DT_F16  1u

@@ -1082,7 +1082,13 @@ __global__ void __launch_bounds__(ChunkCfg<T, C, D>::kThreads, 1)
   // ---- end: every role has left its loop
   umma::tc_fence_before();
   __syncthreads();
-  if (tid == 0 && *abort_flag && a.status) *a.status = 6u;
+  if (*abort_flag) {
+    if (tid == 0 && a.status) *a.status = 6u;
+    // a part that was not finished makes its rows NaN, whatever the workspace held (split items
+    // have one turn: the part is the CTA's number)
+    if (splits > 1 && cta < items)
+      for (int i = tid; i < 256; i += Cfg::kThreads) chunk_ml(work)[(size_t)cta * 256 + i] = make_float2(NAN, NAN);
+  }
   if (warp == 8) {
     umma::tc_fence_after();
     umma::tmem_relinquish();

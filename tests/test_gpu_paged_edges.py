@@ -111,3 +111,37 @@ def test_f32_rows_of_unlike_size_in_one_tile(pkg, torch, new, total, which):
     got, gl, st = attend(pkg, torch, b, q, pool, "f32")
     assert st == 0
     check_on_gpu(torch, b, got, gl, q, pool, "f32", "f32")
+
+
+# ---------------------------------------------------------------- the largest batches
+def test_as_many_single_tokens_as_there_are(pkg, torch):
+    """66,000 sequences of one token over 32 kv heads, one position each: the row is its value."""
+    seqs, heads, d = 66000, 32, 64
+    g = torch.Generator(device="cuda").manual_seed(1)
+    q, out = (torch.randn(seqs, heads * d, generator=g, device="cuda").half() for _ in range(2))
+    kp, vp = (torch.randn(64, heads, 1, d, generator=g, device="cuda").half() for _ in range(2))
+    start = torch.arange(seqs + 1, dtype=torch.int32, device="cuda")
+    length = torch.ones(seqs, dtype=torch.int32, device="cuda")
+    table = (start[:seqs] % 64).contiguous()
+    work = torch.empty(pkg.engine.PAGED_WORK_BYTES, dtype=torch.uint8, device="cuda")
+    st = torch.zeros(1, dtype=torch.int32, device="cuda")
+    pkg.engine.paged_attention(q.data_ptr(), out.data_ptr(), seqs, heads, heads, d, kp.data_ptr(), vp.data_ptr(), 64, 1,
+                               start.data_ptr(), length.data_ptr(), table.data_ptr(), 1, seqs, 1, work.data_ptr(),
+                               dtype="f16", kv_dtype="f16", status_ptr=st.data_ptr())
+    torch.cuda.synchronize()
+    assert int(st.item()) == 0
+    assert torch.equal(out.view(seqs, heads, d), vp[:, :, 0][table.long()])
+
+
+@pytest.mark.parametrize("t,kv", TYPES)
+def test_more_work_than_is_counted_is_out_of_range(pkg, torch, t, kv):
+    """2^30 positions of single tokens: the documented status, nothing computed."""
+    page = 1 << 20
+    b = ref.Batch(np.random.default_rng(0), [1, 1], [page, 100], page, spare=0)
+    b.pages = 1
+    pool = Pool(torch, kv, b, 1, 64, "slot")
+    b.len[0] = 1 << 30
+    b.table, b.wide = np.zeros((2, 1024), np.int32), 1024
+    q = np.ones((2, 4, 64))
+    got, gl, st = attend(pkg, torch, b, q, pool, t)
+    assert st == RANGE and np.all(got == -7.0) and np.all(gl == -7.0)
