@@ -229,6 +229,10 @@ struct ItemRange {
 QORA_DEV int row_token(const AttnArgs& a, int r) { return (r * a.group_inv) >> 16; }
 
 // The sequences' row tiles as a warp holds them: a lane sums a run of neighbouring sequences.
+// Rows that no two sequences share make at most 2^24 / tokens + 2^20 tiles, below kManyTiles; a
+// lane that counts more (overlapping ranges) stays there, so that the warp's sum cannot wrap
+// and the batch is refused as having too many.
+constexpr int kManyTiles = 1 << 25;
 struct ItemMap {
   int per, mine, upto, total;  // sequences of a lane; its row tiles; those up to it; all
 };
@@ -248,7 +252,7 @@ QORA_DEV ItemMap item_map(const AttnArgs& a, int tokens, int lane) {
 #pragma unroll 4
   for (int j = 0; j < m.per; ++j) {
     const int s = lane * m.per + j;
-    if (s < a.batch.seqs) m.mine += seq_tiles(a, s, tokens);
+    if (s < a.batch.seqs) m.mine = min(kManyTiles, m.mine + seq_tiles(a, s, tokens));
   }
   m.upto = m.mine;
 #pragma unroll

@@ -113,6 +113,26 @@ def test_f32_rows_of_unlike_size_in_one_tile(pkg, torch, new, total, which):
     check_on_gpu(torch, b, got, gl, q, pool, "f32", "f32")
 
 
+def test_more_row_tiles_than_32_bits_count(pkg, torch):
+    """Overlapping ranges of 2^24 rows whose tiles add up past 2^31 and 2^32: refused, nothing written."""
+    rows, d = 1 << 24, 64
+    q = torch.zeros(rows, d, dtype=torch.float16, device="cuda")
+    out = torch.full((rows, d), -7.0, dtype=torch.float16, device="cuda")
+    page = torch.zeros(2, 16, d, dtype=torch.float16, device="cuda")
+    work = torch.empty(pkg.engine.PAGED_WORK_BYTES, dtype=torch.uint8, device="cuda")
+    for seqs in (1 << 16, 1 << 17, (1 << 17) + 64, 1 << 20):  # half of them own every row: 2^16 tiles each
+        start = torch.tensor([0, rows], dtype=torch.int32, device="cuda").repeat(seqs // 2 + 1)[:seqs + 1].contiguous()
+        length = torch.full((seqs,), 16, dtype=torch.int32, device="cuda")
+        table = torch.zeros(seqs, dtype=torch.int32, device="cuda")
+        st = torch.zeros(1, dtype=torch.int32, device="cuda")
+        pkg.engine.paged_attention(q.data_ptr(), out.data_ptr(), rows, 1, 1, d, page[0].data_ptr(), page[1].data_ptr(), 1, 16,
+                                   start.data_ptr(), length.data_ptr(), table.data_ptr(), 1, seqs, rows, work.data_ptr(),
+                                   dtype="f16", kv_dtype="f16", status_ptr=st.data_ptr())
+        torch.cuda.synchronize()
+        assert int(st.item()) == RANGE
+        assert bool((out == -7.0).all())
+
+
 # ---------------------------------------------------------------- the largest batches
 def test_as_many_single_tokens_as_there_are(pkg, torch):
     """66,000 sequences of one token over 32 kv heads, one position each: the row is its value."""
