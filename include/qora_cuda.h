@@ -387,7 +387,8 @@ qora_status qora_qk_norm_rope(const void* d_q, uint64_t q_stride, const void* d_
 /* Append the rows' k and v to the pages at their positions, k normalised and rotated on the
  * way as in qora_qk_norm_rope (the position is the one the batch gives the row); q, when
  * q_heads is not 0, goes through the same norm and rotation to d_q_out (which may be d_q).
- * A row whose position is negative (L < n) has no place and is skipped, as out of range.
+ * A row whose position is negative (L < n) has no place and is skipped, as out of range; one
+ * whose page does not exist is not appended, its q is still turned.
  * No two rows may have the same place: two sequences may share pages, but not append to
  * the same slot in one call (which of the rows such a slot then holds is not defined). */
 qora_status qora_paged_append(const void* d_q, uint64_t q_stride, const void* d_k, uint64_t k_stride,

@@ -206,7 +206,7 @@ __global__ void __launch_bounds__(32 * kRowWarps, 4) rows_kernel(const RowArgs a
       return;
     }
     const long long pl = (long long)len - (q1 - q0) + (row - q0);
-    if (pl < 0 || pl >= (long long)a.batch.table_stride * a.pg.page_size) {
+    if (pl < 0 || len > (long long)a.batch.table_stride * a.pg.page_size) {  // pl < len
       if (lane == 0 && a.status) *a.status = 5u;
       return;
     }

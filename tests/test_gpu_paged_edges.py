@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 
 import paged_ref as ref
-from test_gpu_paged import RANGE, TYPES, Pool, attend, check_attention, check_on_gpu, make
+from test_gpu_paged import RANGE, TYPES, Meta, Pool, attend, check_attention, check_on_gpu, dev, host, make, tt
 from test_gpu_paged import torch as torch  # the fixture
 
 pytestmark = pytest.mark.gpu
@@ -165,3 +165,28 @@ def test_more_work_than_is_counted_is_out_of_range(pkg, torch, t, kv):
     q = np.ones((2, 4, 64))
     got, gl, st = attend(pkg, torch, b, q, pool, t)
     assert st == RANGE and np.all(got == -7.0) and np.all(gl == -7.0)
+
+
+@pytest.mark.parametrize("t,kv", TYPES)
+def test_append_of_a_sequence_that_does_not_fit(pkg, torch, t, kv):
+    """A length beyond the table row: nothing of the sequence is appended, not its fitting rows either."""
+    rng = np.random.default_rng(1)
+    b = ref.Batch(rng, [2, 3, 1], [8, 8, 5], 4, wide=2)
+    x = ref.round_to(rng.standard_normal((b.rows, 4, 64)), t)
+    before = [ref.round_to(rng.standard_normal((b.pages, 4, 1, 64)), kv) for _ in range(2)]
+    pool, m = Pool(torch, kv, b, 1, 64, "slot", before), Meta(torch, b)
+    m.len[1] = 9
+    buf = dev(torch, x.reshape(b.rows, -1)).to(tt(torch, t))
+    qo, st = torch.full((b.rows, 128), -7.0, dtype=buf.dtype, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda")
+    at, e = buf.data_ptr(), buf.element_size()
+    pkg.engine.paged_append(at + 128 * e, at + 192 * e, b.rows, 1, 64, **pool.args(), **m.kw, q_ptr=at, q_out_ptr=qo.data_ptr(),
+                            q_heads=2, dtype=t, q_stride=256, k_stride=256, v_stride=256, status_ptr=st.data_ptr())
+    torch.cuda.synchronize()
+    assert int(st.item()) == RANGE
+    want = [z.copy() for z in before]
+    for s, p, row in ((0, 6, 0), (0, 7, 1), (2, 4, 5)):
+        for z, h in zip(want, (2, 3)):
+            z[b.place(s, p)] = ref.round_to(x[row, h], kv)
+    assert all(np.array_equal(u, w) for u, w in zip(pool.values(), want))
+    got = host(qo)
+    assert np.all(got[2:5] == -7.0) and np.array_equal(got[[0, 1, 5]], x[[0, 1, 5], :2].reshape(3, -1))
