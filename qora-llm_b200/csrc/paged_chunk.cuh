@@ -293,7 +293,7 @@ QORA_DEV ItemRange item_at(const AttnArgs& a, const ItemMap& m, int tokens, int 
   const int hi = min(r.len, p0 + r.toks);           // positions [lo, hi) are attended to
   const int lo = first_seen(a, p0);
   r.lo = lo;
-  const int t0 = lo / kPos, nt = max(0, (hi + kPos - 1) / kPos - t0);
+  const int t0 = lo / kPos, nt = hi > lo ? (hi - 1) / kPos + 1 - t0 : 0;
   r.parts = max(1, min(splits, nt));
   if (split >= (unsigned)r.parts) {  // a turn that the item has no use for
     r.toks = r.tiles = 0;
@@ -608,7 +608,7 @@ __global__ void __launch_bounds__(ChunkCfg<T, C, D>::kThreads, 1)
       for (int j = 0; j < it.tiles; ++j) {
         const int tile0 = it.first + j * kPos, ring8 = (tiles + j) & 7;
         if constexpr (!kWide) {
-          if (boxes && tile0 + kPos <= it.len &&
+          if (boxes && kPos <= it.len - tile0 &&
               __all_sync(0xffffffffu, lane >= boxes || (bpage >= 0 && bpage < a.pg.num_pages))) {
             if (np) flush();
             ok = __all_sync(0xffffffffu, ok) != 0;
@@ -1061,7 +1061,7 @@ __global__ void __launch_bounds__(ChunkCfg<T, C, D>::kThreads, 1)
           const int h = it.head * a.group + rr - tok * a.group;
           float o2[D / 32], m2, l2;
           row_attend<T, C, D>(a, static_cast<const T*>(a.q) + row * a.q_stride + h * D, table, it.head, max(first2, it.first),
-                              min(last2, it.first + it.tiles * kPos - 1), scale2, progress, o2, m2, l2);
+                              min(last2, it.first + (it.tiles * kPos - 1)), scale2, progress, o2, m2, l2);
           if (lane == src) {
             m = m2;
             l = l2;

@@ -190,3 +190,23 @@ def test_append_of_a_sequence_that_does_not_fit(pkg, torch, t, kv):
     assert all(np.array_equal(u, w) for u, w in zip(pool.values(), want))
     got = host(qo)
     assert np.all(got[2:5] == -7.0) and np.array_equal(got[[0, 1, 5]], x[[0, 1, 5], :2].reshape(3, -1))
+
+
+@pytest.mark.parametrize("t,kv", TYPES)
+@pytest.mark.parametrize("n", [1, 2, 40, 300])
+def test_positions_up_to_two_to_the_31(pkg, torch, t, kv, n):
+    """The longest sequence a table can describe (one page, named again and again), by a window."""
+    page, wide, window = 42966, 49981, 100
+    L = page * wide
+    assert 2**31 - 128 < L < 2**31
+    rng = np.random.default_rng(n)
+    b = ref.Batch(rng, [n], [page], page, spare=0)
+    q = ref.round_to(rng.standard_normal((b.rows, 2, 64)), t)
+    pages = [ref.round_to(rng.standard_normal((1, page, 1, 64)), kv) for _ in range(2)]
+    pool = Pool(torch, kv, b, 1, 64, "slot", pages)
+    b.len[:] = L
+    b.table, b.wide = np.zeros((1, wide), np.int32), wide
+    got, gl, st = attend(pkg, torch, b, q, pool, t, window=window)
+    assert st == 0
+    b.len[:] = page  # the last positions lie in the page's last slots either way
+    check_attention(b, got, gl, q, pages, t, kv, 0.125, window)
