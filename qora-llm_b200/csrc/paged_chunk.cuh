@@ -93,8 +93,8 @@ struct ChunkCfg {
   static constexpr int kFlush = 4;
 };
 constexpr int kChunkMaxCtas = 160;
-// Longest wait on a barrier, counted from the last progress of a warp that recomputes rows
-// (which takes as long as the rows are long); only a fault reaches it.
+// Longest wait on a barrier, counted from the last mark of a warp that recomputes rows (which
+// takes as long as the rows are long); only a fault reaches it.
 constexpr unsigned long long kWaitNs = 2000000000ull;
 
 constexpr int kChunkMaxParts = kChunkMaxCtas;  // parts of split items in one call: no more than CTAs
@@ -307,10 +307,10 @@ QORA_DEV ItemRange item_at(const AttnArgs& a, const ItemMap& m, int tokens, int 
   return r;
 }
 
-// A row by one warp, over positions [from, to]: lane's elements lane + 32 i. Raises `progress`.
+// A row by one warp, over positions [from, to]: lane's elements lane + 32 i. Renews `mark`.
 template <typename T, typename C, int D>
 QORA_DEV void row_attend(const AttnArgs& a, const T* q, const int* table, int head, int from, int to, float scale2,
-                         unsigned* progress, float (&o)[D / 32], float& m, float& l) {
+                         volatile uint64_t* mark, float (&o)[D / 32], float& m, float& l) {
   const int lane = threadIdx.x & 31;
   float qv[D / 32];
   for (int i = 0; i < D / 32; ++i) {
@@ -321,7 +321,7 @@ QORA_DEV void row_attend(const AttnArgs& a, const T* q, const int* table, int he
   l = 0.0f;
 #pragma unroll 1
   for (int j = from; j <= to; ++j) {
-    if ((j & 63) == 0 && lane == 0) atomicAdd(progress, 1u);
+    if ((j & 63) == 0 && lane == 0) *mark = ptx::globaltimer();
     const int pi = j / a.pg.page_size, page = table[pi];
     if (page < 0 || page >= a.pg.num_pages) continue;
     const long long off = page * a.pg.page_stride + (long long)(j - pi * a.pg.page_size) * a.pg.slot_stride +
@@ -390,7 +390,7 @@ __global__ void __launch_bounds__(ChunkCfg<T, C, D>::kThreads, 1)
   uint32_t* const s_low = s_max + 8;                                // [K, V][4 warps]
   uint32_t* const s_tmem = s_low + 8;
   volatile int* const abort_flag = reinterpret_cast<volatile int*>(s_tmem + 1);
-  uint32_t* const progress = s_tmem + 2;
+  volatile uint64_t* const mark = reinterpret_cast<volatile uint64_t*>(s_tmem + 2);
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int block_toks = Cfg::kBlock / a.group, tokens = 2 * block_toks;
@@ -409,7 +409,7 @@ __global__ void __launch_bounds__(ChunkCfg<T, C, D>::kThreads, 1)
     }
     ptx::mbar_init(done, 1);
     *abort_flag = 0;
-    *progress = 0;
+    *mark = 0;
     ptx::fence_mbar_init();
   }
   if (warp == 8) umma::tmem_alloc(s_tmem, 512);
@@ -432,7 +432,7 @@ __global__ void __launch_bounds__(ChunkCfg<T, C, D>::kThreads, 1)
   auto item_of = [&](int w) { return w * ctas + (w & 1 ? ctas - 1 - cta : cta); };
   // whether a block's numerators begin anew with tile j
   auto fresh = [&](int j) { return j == 0 || (kHalves && j % Cfg::kFlush == 0); };
-  auto wait = [&](uint64_t* bar, uint32_t parity) { return umma::wait_bar(bar, parity, kWaitNs, abort_flag, progress); };
+  auto wait = [&](uint64_t* bar, uint32_t parity) { return umma::wait_bar(bar, parity, kWaitNs, abort_flag, mark); };
 
   if (warp == 8) {
     // -------------------------------------------------------------------- products
@@ -1061,7 +1061,7 @@ __global__ void __launch_bounds__(ChunkCfg<T, C, D>::kThreads, 1)
           const int h = it.head * a.group + rr - tok * a.group;
           float o2[D / 32], m2, l2;
           row_attend<T, C, D>(a, static_cast<const T*>(a.q) + row * a.q_stride + h * D, table, it.head, max(first2, it.first),
-                              min(last2, it.first + (it.tiles * kPos - 1)), scale2, progress, o2, m2, l2);
+                              min(last2, it.first + (it.tiles * kPos - 1)), scale2, mark, o2, m2, l2);
           if (lane == src) {
             m = m2;
             l = l2;

@@ -1,6 +1,6 @@
 // The bounded waits of tcgen05.cuh on a GPU, each with a limit of a few milliseconds: a wait
-// whose partner reports progress outlasts the limit and ends when the barrier completes; one
-// without progress gives up, sets the abort flag and returns. Settling waits for copies in
+// whose partner renews the mark outlasts the limit and ends when the barrier completes; one
+// that is not renewed gives up, sets the abort flag and returns. Settling waits for copies in
 // flight and has a limit too. Prints "ok".
 #include <cstdio>
 
@@ -10,22 +10,22 @@ using namespace qora;
 
 constexpr unsigned long long kLimit = 3000000;  // ns
 
-// Thread 0 waits; thread 32 raises the counter every limit / 10 for `rounds`, then arrives
+// Thread 0 waits; thread 32 renews the mark every limit / 10 for `rounds`, then arrives
 // (arrive != 0) or leaves the barrier as it is.
 __global__ void wait_kernel(int rounds, int arrive, int counted, int* out) {
   __shared__ uint64_t bar;
   __shared__ volatile int abort_flag;
-  __shared__ volatile unsigned progress;
+  __shared__ volatile uint64_t mark;
   if (threadIdx.x == 0) {
     ptx::mbar_init(&bar, 1);
     ptx::fence_mbar_init();
     abort_flag = 0;
-    progress = 0;
+    mark = 0;
   }
   __syncthreads();
   if (threadIdx.x == 0) {
     const uint64_t t0 = ptx::globaltimer();
-    out[0] = umma::wait_bar(&bar, 0, kLimit, &abort_flag, counted ? &progress : nullptr);
+    out[0] = umma::wait_bar(&bar, 0, kLimit, &abort_flag, counted ? &mark : nullptr);
     out[1] = abort_flag;
     out[2] = (int)((ptx::globaltimer() - t0) / 1000);  // us
   } else if (threadIdx.x == 32) {
@@ -33,7 +33,7 @@ __global__ void wait_kernel(int rounds, int arrive, int counted, int* out) {
       const uint64_t t0 = ptx::globaltimer();
       while (ptx::globaltimer() - t0 < kLimit / 10) {
       }
-      progress = progress + 1;
+      mark = ptx::globaltimer();
     }
     if (arrive) ptx::mbar_arrive(&bar);
   }
@@ -69,7 +69,7 @@ int main() {
   struct Case {
     int rounds, arrive, counted, ended, least_us;
   };
-  // five limits of work with progress; the same unseen; progress that stops; at once
+  // five limits of work with marks; the same unseen; marks that stop; at once
   const Case cases[] = {{50, 1, 1, 1, 10000}, {50, 1, 0, 0, 2900}, {20, 0, 1, 0, 8000}, {0, 1, 1, 1, 0}};
   for (const Case& c : cases) {
     wait_kernel<<<1, 64>>>(c.rounds, c.arrive, c.counted, out);
