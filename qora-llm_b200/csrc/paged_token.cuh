@@ -310,11 +310,9 @@ __global__ void __launch_bounds__(32 * TokenCfg<T, C, D>::kWarps, 1) token_kerne
     auto issue = [&](int step, int stage, int page) {  // page: of position step * kPos + lane
       constexpr int kHop = 32 / kChunks;
       const int pos = sw.first + step * kPos;
-      const int left = sw.len - pos;  // positions that there are from here on
       const uint32_t dk = ptx::smem_addr(ring + stage * Cfg::kStep), dv = dk + Cfg::kSide;
-      const unsigned ahead = pos < sw.lo ? (1u << (sw.lo - pos)) - 1 : 0u;  // not attended to (first step)
-      const unsigned gone = (left >= kPos ? 0u : ~0u << max(0, left) & ((1u << kPos) - 1)) | ahead;
-      const long long off = offset_of(pos + (lane & (kPos - 1)), page);
+      const int mine = pos + (lane & (kPos - 1));
+      const long long off = offset_of(mine, page);
       const unsigned bad = __ballot_sync(0xffffffffu, off < 0) & ((1u << kPos) - 1);
 #pragma unroll
       for (int i = 0; i < kPos / kHop; ++i) {
@@ -323,10 +321,8 @@ __global__ void __launch_bounds__(32 * TokenCfg<T, C, D>::kWarps, 1) token_kerne
         cp_async_16(dk + Cfg::k_at(crow + i * kHop, cch), kbase + at, o >= 0);
         cp_async_16(dv + Cfg::v_at(crow + i * kHop, cch), vbase + at, o >= 0);
       }
-      if (lane == 0) {
-        s_bad[warp][stage] = bad;
-        if (a.status && (bad & ~gone)) *a.status = 5u;  // a page that does not exist
-      }
+      if (lane == 0) s_bad[warp][stage] = bad;
+      if (bad && a.status && off < 0 && mine >= sw.lo && mine < sw.len) *a.status = 5u;  // a page that does not exist
     };
 
     // q in the instruction's layout. f32 rows: 2^e puts the row's largest value in [2^13, 2^14)
