@@ -24,7 +24,8 @@
 // Values that are masked never count: masked scores become -inf, slots behind the last
 // position are filled with zeros. What a weight of zero times an infinite value leaves (NaN)
 // shows in the numerators; such a segment is run again with the non-finite elements of V
-// taken out and added to the rows that do see them.
+// taken out and added to the rows that do see them, and with NaN scores of f32 rows (an
+// infinite key's product with halves of unlike sign) computed in f32.
 //
 // Measured (graph replays, pages of 16): 128 tokens over up to 4,100 binary16 positions, 1.1
 // GB, 174 us = 6.3 TB/s; 32 tokens over f32 caches, 253 MB, 54 us = 4.7 TB/s; one token over
@@ -401,6 +402,18 @@ __global__ void __launch_bounds__(32 * TokenCfg<T, C, D>::kWarps, 1) token_kerne
       __syncthreads();
     };
 
+    // f32 rows: q . k in f32, of the thread's row and position `w` of a step. An infinite value
+    // leaves NaN in the sum of products of halves, where q . k may be infinite.
+    auto plain_score = [&](const uint8_t* pk, int w) {
+      const float* q = reinterpret_cast<const float*>(row_ptr(g < nrows ? g : 0));
+      constexpr int kPiece = 16 / (int)sizeof(C);
+      float d = 0.0f;
+#pragma unroll 1
+      for (int x = 0; x < D; ++x)
+        d = __fmaf_rn(q[x], to_f32(reinterpret_cast<const C*>(pk + Cfg::k_at(w, x / kPiece))[x % kPiece]), d);
+      return d;
+    };
+
     constexpr int kO = D / 8;  // numerators: n8 tiles of 4 values
     float o[kO][4];
     float m[2], l[2];
@@ -503,6 +516,16 @@ __global__ void __launch_bounds__(32 * TokenCfg<T, C, D>::kWarps, 1) token_kerne
               s[n][2 * r + j] = x;
               mx[r] = fmaxf(mx[r], x);
             }
+        if (kHalves && careful) {
+#pragma unroll
+          for (int n = 0; n < kN; ++n)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+              if (s[n][j] != s[n][j]) {
+                s[n][j] = plain_score(pk, 8 * n + 2 * t + j) * scale2;
+                mx[0] = fmaxf(mx[0], s[n][j]);
+              }
+        }
         bool raise = false;
 #pragma unroll
         for (int r = 0; r < kR; ++r) {

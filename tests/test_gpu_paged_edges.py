@@ -210,3 +210,41 @@ def test_positions_up_to_two_to_the_31(pkg, torch, t, kv, n):
     assert st == 0
     b.len[:] = page  # the last positions lie in the page's last slots either way
     check_attention(b, got, gl, q, pages, t, kv, 0.125, window)
+
+
+# ---------------------------------------------------------------- infinite keys
+@pytest.mark.parametrize("t,kv", TYPES)
+@pytest.mark.parametrize("new,total,hq", [([1], [300], 4), ([2, 1], [90, 700], 2), ([3], [70], 4), ([64], [200], 4)])
+def test_a_score_of_minus_infinity_has_no_weight(pkg, torch, t, kv, new, total, hq):
+    """An infinite key whose scores are -inf: its position has no weight, the row is finite. Where
+    one score is +inf, and where one is inf - inf, the row is NaN."""
+    rng = np.random.default_rng(15)
+    b, q, pages, _ = make(torch, rng, t, kv, new, total, 16, "head", hq, 1, 64, qmul=0.5)
+    q[:, :, 3] = ref.round_to(0.3 + np.abs(q[:, :, 3]), t)
+    q[:, :, 11] = ref.round_to(-0.7 - np.abs(q[:, :, 11]), t)
+    at = [b.place(s, p) for s in range(b.seqs) for p in (total[s] // 3, total[s] - new[s])]
+    for i, (pg, sl) in enumerate(at):
+        pages[0][pg, sl, 0, 3 if i % 2 else 11] = -np.inf if i % 2 else np.inf  # scores of -inf for every row
+    got, gl, st = attend(pkg, torch, b, q, Pool(torch, kv, b, 1, 64, "head", pages), t)
+    assert st == 0
+    hidden = [pages[0].copy(), pages[1]]
+    for pg, sl in at:
+        hidden[0][pg, sl, 0] = 0.0
+    size = ref.attention(b, q, *hidden, 0.125, 0)[3]  # of the positions that count
+    with np.errstate(invalid="ignore"):
+        out, wl, mass, _ = ref.attention(b, q, *pages, 0.125, 0)
+    bound, lb = ref.attention_bounds(b, out, mass, size, t, kv, 64)
+    rows = int(b.start[-1])
+    assert np.isfinite(out[:rows]).all()
+    assert np.all(np.abs(got - out)[:rows] <= bound[:rows])
+    assert np.all(np.abs(gl - wl)[:rows] <= (lb + 2.0**-23 * np.abs(wl))[:rows])
+    pg, sl = at[1]
+    for key in ([(3, np.inf)], [(3, np.inf), (11, np.inf)]):  # +inf; inf - inf
+        two = pages[0].copy()
+        for d, v in key:
+            two[pg, sl, 0, d] = v
+        got, gl, st = attend(pkg, torch, b, q, Pool(torch, kv, b, 1, 64, "head", [two, pages[1]]), t)
+        last = slice(0, b.new[0])  # every new row of sequence 0 sees it
+        assert np.isnan(got[last]).all() and np.isnan(gl[last]).all()
+        other = slice(b.new[0], rows)
+        assert np.all(np.abs(got - out)[other] <= bound[other])
