@@ -41,10 +41,13 @@
 // The running maximum is raised only when it grows by more than 2^kSlack: then the
 // numerators in TMEM are scaled, which is rare after the first tiles. Masked scores become
 // -inf before the maximum. Rows that meet a non-finite value (a weight of zero times an
-// infinite value of V, or a row whose own scores are) are computed again by one warp, one
-// position at a time (row_attend). So are rows of an f32 cache that meet a tile of K or V
-// whose rows differ by more than 2^14 in size, a tile of V 2^12 below the largest before
-// it, or growth of V by more than 2^60.
+// infinite value of V, or a row whose own scores are) are computed again in f32 when the CTA's
+// roles have ended (rows_attend). So are rows of an f32 cache that meet a tile of K or V whose
+// rows differ by more than 2^14 in size, a tile of V 2^12 below the largest before it, or
+// growth of V by more than 2^60. This is for correctness alone, and 15 to 70 times as slow:
+// where every row is concerned, 1,021 f32 rows take 0.85 ms instead of 56 us, 512 f32 rows
+// over 8,192 binary16 positions 4.4 ms, 2,048 binary16 rows 4.2 ms instead of 42 us (one row
+// and one position at a time, between the tiles, took 10, 41 and 40 ms).
 //
 // Measured, 16 query heads over 4 kv heads of 128: a prompt of 8,192 binary16 rows in 264 to
 // 272 us = 1.01 to 1.04 PFLOP/s of 275 GFLOP; 512 f32 rows over 8,192 binary16 positions in
@@ -93,8 +96,11 @@ struct ChunkCfg {
   static constexpr int kFlush = 4;
 };
 constexpr int kChunkMaxCtas = 160;
-// Longest wait on a barrier, counted from the last mark of a warp that recomputes rows (which
-// takes as long as the rows are long); only a fault reaches it.
+// Turns of a CTA whose marks for recomputing are told apart; one more turn shares the mark of the
+// first, and the rows of both are computed again.
+constexpr int kRedoTurns = 512;
+// Longest wait on a barrier; only a fault reaches it. (Rows are recomputed, which takes as long
+// as the rows are long, when the CTA's roles have ended and nothing waits.)
 constexpr unsigned long long kWaitNs = 2000000000ull;
 
 constexpr int kChunkMaxParts = kChunkMaxCtas;  // parts of split items in one call: no more than CTAs
@@ -307,37 +313,102 @@ QORA_DEV ItemRange item_at(const AttnArgs& a, const ItemMap& m, int tokens, int 
   return r;
 }
 
-// A row by one warp, over positions [from, to]: lane's elements lane + 32 i. Renews `mark`.
+// Up to four rows of one kv head by a warp, in f32: row r over positions [from[r], to[r]], all
+// within [lo, hi]; o[r]: lane's elements lane * D / 32 + i. Four positions at a time: K and V
+// are read once for the four rows, and the 16 dot products are added up over the lanes
+// together (lane / 8: row, lane / 2 % 4: position).
+template <typename T, int E>
+struct alignas(E * sizeof(T)) Piece {
+  T v[E];
+};
 template <typename T, typename C, int D>
-QORA_DEV void row_attend(const AttnArgs& a, const T* q, const int* table, int head, int from, int to, float scale2,
-                         volatile uint64_t* mark, float (&o)[D / 32], float& m, float& l) {
-  const int lane = threadIdx.x & 31;
-  float qv[D / 32];
-  for (int i = 0; i < D / 32; ++i) {
-    qv[i] = to_f32(q[lane + 32 * i]);
-    o[i] = 0.0f;
+QORA_DEV void rows_attend(const AttnArgs& a, const T* const (&q)[4], const int (&from)[4], const int (&to)[4],
+                          int lo, int hi, const int* table, int head, float scale2,
+                          float (&o)[4][D / 32], float& m, float& l) {
+  constexpr int E = D / 32, R = 4, P = 4;
+  const int lane = threadIdx.x & 31, mine = lane >> 3, which = (lane >> 1) & 3;
+  float qv[R][E];
+  int first = from[0], last = to[0];  // of the lane's row
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const Piece<T, E> x = *reinterpret_cast<const Piece<T, E>*>(q[r] + lane * E);
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      qv[r][e] = to_f32(x.v[e]);
+      o[r][e] = 0.0f;
+    }
+    if (mine == r) first = from[r], last = to[r];
   }
   m = -INFINITY;
   l = 0.0f;
 #pragma unroll 1
-  for (int j = from; j <= to; ++j) {
-    if ((j & 63) == 0 && lane == 0) *mark = ptx::globaltimer();
-    const int pi = j / a.pg.page_size, page = table[pi];
-    if (page < 0 || page >= a.pg.num_pages) continue;
-    const long long off = page * a.pg.page_stride + (long long)(j - pi * a.pg.page_size) * a.pg.slot_stride +
-                          (long long)head * a.pg.head_stride;
-    const C* k = static_cast<const C*>(a.k_pages) + off;
-    const C* v = static_cast<const C*>(a.v_pages) + off;
-    float d = 0.0f;
-    for (int i = 0; i < D / 32; ++i) d = __fmaf_rn(qv[i], to_f32(k[lane + 32 * i]), d);
-    d = __fmul_rn(warp_sum(d), scale2);
-    const float mn = fmaxf(m, d);
-    const float mu = mn == -INFINITY ? 0.0f : mn;  // a NaN score does not raise the maximum: its weight is NaN
-    const float w = exp2f(d - mu + kShift), c = exp2f(m - mu);
-    l = __fmaf_rn(l, c, w);
-    for (int i = 0; i < D / 32; ++i) o[i] = __fmaf_rn(o[i], c, w == 0.0f ? 0.0f : __fmul_rn(w, to_f32(v[lane + 32 * i])));
-    m = mn;
+  for (int base = lo; base <= hi; base += min(32, hi - base + 1)) {
+    long long off = -1;
+    if (lane <= hi - base) {
+      const int pos = base + lane, pi = pos / a.pg.page_size, page = table[pi];
+      if (page >= 0 && page < a.pg.num_pages)
+        off = page * a.pg.page_stride + (long long)(pos - pi * a.pg.page_size) * a.pg.slot_stride + (long long)head * a.pg.head_stride;
+    }
+    const unsigned there = __ballot_sync(0xffffffffu, off >= 0);
+#pragma unroll 1
+    for (int j = 0; j < 32 && j <= hi - base; j += P) {
+      Piece<C, E> k[P], v[P];
+      float s[R * P];
+#pragma unroll
+      for (int x = 0; x < P; ++x) {
+        const long long at = __shfl_sync(0xffffffffu, off, j + x);
+        k[x] = v[x] = Piece<C, E>{};
+        if (at >= 0) {
+          k[x] = *reinterpret_cast<const Piece<C, E>*>(static_cast<const C*>(a.k_pages) + at + lane * E);
+          v[x] = *reinterpret_cast<const Piece<C, E>*>(static_cast<const C*>(a.v_pages) + at + lane * E);
+        }
+      }
+#pragma unroll
+      for (int x = 0; x < P; ++x)
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          float d = 0.0f;
+#pragma unroll
+          for (int e = 0; e < E; ++e) d = __fmaf_rn(qv[r][e], to_f32(k[x].v[e]), d);
+          s[P * r + x] = d;
+        }
+      // halving the number of sums while doubling the lanes that each of them covers
+#pragma unroll
+      for (int n = 8; n > 0; n >>= 1) {
+        const bool up = lane & (2 * n);
+#pragma unroll
+        for (int i = 0; i < n; ++i) {
+          const float give = up ? s[i] : s[i + n], keep = up ? s[i + n] : s[i];
+          s[i] = __fadd_rn(keep, __shfl_xor_sync(0xffffffffu, give, 2 * n));
+        }
+      }
+      float d = __fmul_rn(__fadd_rn(s[0], __shfl_xor_sync(0xffffffffu, s[0], 1)), scale2);
+      const int pos = base + j + which;
+      if (!((there >> (j + which)) & 1) || pos < first || pos > last) d = -INFINITY;
+      float top = fmaxf(d, __shfl_xor_sync(0xffffffffu, d, 2));
+      top = fmaxf(m, fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4)));
+      const float mu = top == -INFINITY ? 0.0f : top;  // a NaN score does not raise the maximum: its weight is NaN
+      const float w = exp2f(d - mu + kShift), c = exp2f(m - mu);
+      m = top;
+      l = __fmaf_rn(l, c, w);
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const float cr = __shfl_sync(0xffffffffu, c, 8 * r);
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[r][e] *= cr;
+#pragma unroll
+        for (int x = 0; x < P; ++x) {
+          const float wx = __shfl_sync(0xffffffffu, w, 8 * r + 2 * x);
+          if (wx != 0.0f) {  // the same for the whole warp
+#pragma unroll
+            for (int e = 0; e < E; ++e) o[r][e] = __fmaf_rn(wx, to_f32(v[x].v[e]), o[r][e]);
+          }
+        }
+      }
+    }
   }
+  l = __fadd_rn(l, __shfl_xor_sync(0xffffffffu, l, 2));
+  l = __fadd_rn(l, __shfl_xor_sync(0xffffffffu, l, 4));
 }
 
 // Four consecutive f32 values, scaled, as binary16 upper and lower halves.
@@ -390,7 +461,7 @@ __global__ void __launch_bounds__(ChunkCfg<T, C, D>::kThreads, 1)
   uint32_t* const s_low = s_max + 8;                                // [K, V][4 warps]
   uint32_t* const s_tmem = s_low + 8;
   volatile int* const abort_flag = reinterpret_cast<volatile int*>(s_tmem + 1);
-  volatile uint64_t* const mark = reinterpret_cast<volatile uint64_t*>(s_tmem + 2);
+  uint32_t* const s_redo = s_tmem + 2;  // [kRedoTurns / 4] softmax warps whose rows are computed again, a byte per turn
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int block_toks = Cfg::kBlock / a.group, tokens = 2 * block_toks;
@@ -409,9 +480,9 @@ __global__ void __launch_bounds__(ChunkCfg<T, C, D>::kThreads, 1)
     }
     ptx::mbar_init(done, 1);
     *abort_flag = 0;
-    *mark = 0;
     ptx::fence_mbar_init();
   }
+  for (int i = tid; i < kRedoTurns / 4; i += Cfg::kThreads) s_redo[i] = 0u;
   if (warp == 8) umma::tmem_alloc(s_tmem, 512);
   const ItemMap map = item_map(a, tokens, lane);
   umma::tc_fence_before();
@@ -432,7 +503,7 @@ __global__ void __launch_bounds__(ChunkCfg<T, C, D>::kThreads, 1)
   auto item_of = [&](int w) { return w * ctas + (w & 1 ? ctas - 1 - cta : cta); };
   // whether a block's numerators begin anew with tile j
   auto fresh = [&](int j) { return j == 0 || (kHalves && j % Cfg::kFlush == 0); };
-  auto wait = [&](uint64_t* bar, uint32_t parity) { return umma::wait_bar(bar, parity, kWaitNs, abort_flag, mark); };
+  auto wait = [&](uint64_t* bar, uint32_t parity) { return umma::wait_bar(bar, parity, kWaitNs, abort_flag); };
 
   if (warp == 8) {
     // -------------------------------------------------------------------- products
@@ -1049,32 +1120,7 @@ __global__ void __launch_bounds__(ChunkCfg<T, C, D>::kThreads, 1)
           if ((fb >> (4 * q)) & 15u) redo |= 1u << (16 * h + 8 + q);
         }
       }
-      // rows to compute again, one after the other by the whole warp
-      redo &= live_rows;
-      if (redo) {
-        __syncwarp();  // other lanes have stored what is stored again here
-        const int* table = a.batch.table + (long long)it.seq * a.batch.table_stride;
-        for (; redo; redo &= redo - 1) {
-          const int src = __ffs(redo) - 1, rr = r0 + src, tok = row_token(a, rr);
-          const int last2 = __shfl_sync(0xffffffffu, plast, src), first2 = __shfl_sync(0xffffffffu, pfirst, src);
-          const long long row = row0 + tok;
-          const int h = it.head * a.group + rr - tok * a.group;
-          float o2[D / 32], m2, l2;
-          row_attend<T, C, D>(a, static_cast<const T*>(a.q) + row * a.q_stride + h * D, table, it.head, max(first2, it.first),
-                              min(last2, it.first + (it.tiles * kPos - 1)), scale2, mark, o2, m2, l2);
-          if (lane == src) {
-            m = m2;
-            l = l2;
-          }
-          const float inv = l2 == 0.0f ? 0.0f : __fdiv_rn(1.0f, l2);
-          for (int i = 0; i < D / 32; ++i) {
-            if (it.part < 0)
-              static_cast<T*>(a.out)[row * a.out_stride + h * D + lane + 32 * i] = from_f32(__fmul_rn(o2[i], inv), T());
-            else
-              chunk_num(work)[((size_t)it.part * 256 + x * 128 + rr) * D + lane + 32 * i] = o2[i];
-          }
-        }
-      }
+      if ((redo & live_rows) && lane == 0) atomicOr(s_redo + w % kRedoTurns / 4, 1u << (w % 4 * 8 + warp));
       if (live) {
         if (it.part >= 0)
           chunk_ml(work)[(size_t)it.part * 256 + x * 128 + r] = make_float2(m, l);
@@ -1086,17 +1132,77 @@ __global__ void __launch_bounds__(ChunkCfg<T, C, D>::kThreads, 1)
   // ---- end: every role has left its loop
   umma::tc_fence_before();
   __syncthreads();
+  if (warp == 8) {
+    umma::tc_fence_after();
+    umma::tmem_relinquish();
+    umma::tmem_dealloc(tmem, 512);
+  }
   if (*abort_flag) {
     if (tid == 0 && a.status) *a.status = 6u;
     // a part that was not finished makes its rows NaN, whatever the workspace held (split items
     // have one turn: the part is the CTA's number)
     if (splits > 1 && cta < items)
       for (int i = tid; i < 256; i += Cfg::kThreads) chunk_ml(work)[(size_t)cta * 256 + i] = make_float2(NAN, NAN);
+    return;
   }
-  if (warp == 8) {
-    umma::tc_fence_after();
-    umma::tmem_relinquish();
-    umma::tmem_dealloc(tmem, 512);
+  // ---- rows to compute again: all of a softmax warp's 32, four at a time, by any warp
+  for (int w = 0; w * ctas < items; ++w) {
+    const uint32_t flags = (s_redo[w % kRedoTurns / 4] >> (w % 4 * 8)) & 0xffu;
+    const int idx = item_of(w);
+    if (!flags || idx >= items) continue;
+    const ItemRange it = item_at<kPos>(a, map, tokens, splits, idx, lane);
+    const int* table = a.batch.table + (long long)it.seq * a.batch.table_stride;
+    const int end = it.first + (it.tiles * kPos - 1);  // the part's last position
+    int turn = 0;
+#pragma unroll 1
+    for (int u = 0; u < 64; ++u) {
+      if (!((flags >> (u >> 3)) & 1) || turn++ % (Cfg::kThreads / 32) != warp) continue;
+      const int x = u >> 5, first_row = (u & 31) * 4;  // of block x
+      const int toks = min(block_toks, it.toks - x * block_toks);
+      const int p0 = it.len - it.n + it.tok0 + x * block_toks;
+      const long long row0 = it.q0 + it.tok0 + x * block_toks;
+      int from[4], to[4], lo = end, hi = -1;
+      long long at[4];  // (row, query head) of the output, or -1
+      const T* q[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int tok = row_token(a, first_row + i);
+        const bool live = tok < toks;
+        const long long row = row0 + (live ? tok : 0);
+        const int h = it.head * a.group + (live ? first_row + i - tok * a.group : 0);
+        q[i] = static_cast<const T*>(a.q) + row * a.q_stride + h * D;
+        at[i] = live ? row * a.hq + h : -1;
+        from[i] = max(first_seen(a, p0 + tok), it.first);
+        to[i] = live ? min(p0 + tok, end) : -1;
+        if (to[i] >= from[i]) lo = min(lo, from[i]), hi = max(hi, to[i]);
+      }
+      if (toks <= 0) continue;
+      float o[4][D / 32], m, l;
+      rows_attend<T, C, D>(a, q, from, to, lo, hi, table, it.head, a.scale * kLog2e, o, m, l);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float mi = __shfl_sync(0xffffffffu, m, 8 * i), li = __shfl_sync(0xffffffffu, l, 8 * i);
+        if (at[i] < 0) continue;
+        const int h = it.head * a.group + first_row + i - row_token(a, first_row + i) * a.group;
+        const long long row = row0 + row_token(a, first_row + i);
+        const size_t part_row = (size_t)max(it.part, 0) * 256 + x * 128 + first_row + i;
+        const float inv = li == 0.0f ? 0.0f : __fdiv_rn(1.0f, li);
+#pragma unroll
+        for (int e = 0; e < D / 32; ++e) {
+          const int d = lane * (D / 32) + e;
+          if (it.part < 0)
+            static_cast<T*>(a.out)[row * a.out_stride + h * D + d] = from_f32(__fmul_rn(o[i][e], inv), T());
+          else
+            chunk_num(work)[part_row * D + d] = o[i][e];
+        }
+        if (lane == 0) {
+          if (it.part >= 0)
+            chunk_ml(work)[part_row] = make_float2(mi, li);
+          else if (a.lse)
+            a.lse[at[i]] = li == 0.0f ? -INFINITY : (mi - kShift + log2f(li)) * kLn2;
+        }
+      }
+    }
   }
 }
 

@@ -43,22 +43,14 @@ QORA_DEV void tmem_ld8(uint32_t taddr, uint32_t (&v)[8]) {
 }
 QORA_DEV void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
-// bounded mbarrier wait; false (and the CTA's abort flag set) after limit_ns. `mark` (shared
-// memory, or null): the time at which a warp that does work of unbounded length last said so;
-// the limit counts from there if that is later. It is looked at when the limit is over: a wait
-// that counts changes as it goes takes 8,192 binary16 rows from 265 to 269 us.
-QORA_DEV bool wait_bar(uint64_t* bar, uint32_t parity, unsigned long long limit_ns, volatile int* abort,
-                       volatile uint64_t* mark = nullptr) {
+// bounded mbarrier wait; false (and the CTA's abort flag set) after limit_ns
+QORA_DEV bool wait_bar(uint64_t* bar, uint32_t parity, unsigned long long limit_ns, volatile int* abort) {
   if (ptx::mbar_try_wait(bar, parity)) return true;
-  uint64_t t0 = ptx::globaltimer();
+  const uint64_t t0 = ptx::globaltimer();
   for (;;) {
     if (ptx::mbar_try_wait(bar, parity)) return true;
     if (*abort) return false;
     if (ptx::globaltimer() - t0 > limit_ns) {
-      if (mark && *mark > t0) {
-        t0 = *mark;
-        continue;
-      }
       *abort = 1;
       return false;
     }

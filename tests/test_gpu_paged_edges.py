@@ -113,6 +113,45 @@ def test_f32_rows_of_unlike_size_in_one_tile(pkg, torch, new, total, which):
     check_on_gpu(torch, b, got, gl, q, pool, "f32", "f32")
 
 
+def test_rows_computed_again_where_a_cta_has_many_items(pkg, torch):
+    """76,800 items, some 519 per CTA: the marks of the first and the last share a place."""
+    seqs, n, heads, d = 1200, 17, 64, 64
+    g = torch.Generator(device="cuda").manual_seed(7)
+    q, k, v = (torch.randn(seqs, n, heads, d, generator=g, device="cuda").half() for _ in range(3))
+    hit = torch.tensor([0, 1, 600, seqs - 2, seqs - 1], device="cuda")
+    v[hit, 3, 7, 9] = float("inf")
+    out = torch.full_like(q, -7.0)
+    lse = torch.full((seqs * n, heads), -7.0, device="cuda")
+    start = torch.arange(0, seqs * n + 1, n, dtype=torch.int32, device="cuda")
+    length = torch.full((seqs,), n, dtype=torch.int32, device="cuda")
+    table = torch.arange(seqs, dtype=torch.int32, device="cuda")
+    work = torch.empty(pkg.engine.PAGED_WORK_BYTES, dtype=torch.uint8, device="cuda")
+    st = torch.zeros(1, dtype=torch.int32, device="cuda")
+    pkg.engine.paged_attention(q.data_ptr(), out.data_ptr(), seqs * n, heads, heads, d, k.data_ptr(), v.data_ptr(), seqs, n,
+                               start.data_ptr(), length.data_ptr(), table.data_ptr(), 1, seqs, n, work.data_ptr(),
+                               lse_ptr=lse.data_ptr(), dtype="f16", kv_dtype="f16", page_strides=(n * heads * d, d, heads * d),
+                               status_ptr=st.data_ptr())
+    torch.cuda.synchronize()
+    assert int(st.item()) == 0
+    reach = torch.zeros(out.shape, dtype=torch.bool, device="cuda")
+    reach[hit, 3:, 7, 9] = True
+    assert torch.equal(torch.isposinf(out), reach) and not torch.isnan(out).any()
+    hide = torch.ones(n, n, dtype=torch.bool, device="cuda").triu(1)
+    b = ref.Batch(np.random.default_rng(0), [n], [n], n)
+    v[hit, 3, 7, 9] = 0.0
+    for s in range(0, seqs, 100):
+        q64, k64, v64 = (z[s:s + 100].double() for z in (q, k, v))
+        x = (torch.einsum("sihd,sjhd->shij", q64, k64) * d ** -0.5).masked_fill(hide, -torch.inf)
+        w = torch.softmax(x, -1)
+        want, mass = (torch.einsum("shij,sjhd->sihd", w, z) for z in (v64, v64.abs()))
+        size = (torch.einsum("sihd,sjhd->shij", q64.abs(), k64.abs()) * d ** -0.5).masked_fill(hide, 0).amax(-1).transpose(1, 2)
+        bound, lb = ref.attention_bounds(b, want.cpu().numpy(), mass.cpu().numpy(), size.cpu().numpy(), "f16", "f16", d)
+        got = torch.where(reach[s:s + 100], want, out[s:s + 100].double())
+        assert np.all((got - want).abs().cpu().numpy() <= bound)
+        wl = torch.logsumexp(x, -1).transpose(1, 2).cpu().numpy()
+        assert np.all(np.abs(host(lse.view(seqs, n, heads)[s:s + 100]) - wl) <= lb + 2.0**-23 * np.abs(wl))
+
+
 def test_more_row_tiles_than_32_bits_count(pkg, torch):
     """Overlapping ranges of 2^24 rows whose tiles add up past 2^31 and 2^32: refused, nothing written."""
     rows, d = 1 << 24, 64

@@ -24,6 +24,6 @@ def test_wait_check_compiles(tmp_path):
 
 
 @pytest.mark.gpu
-def test_waits_see_marks_and_give_up_without(tmp_path):
+def test_waits_give_up_and_settle(tmp_path):
     out = subprocess.run([str(build(tmp_path))], capture_output=True, text=True, timeout=120)
     assert out.returncode == 0 and out.stdout.strip() == "ok", out.stdout + out.stderr
