@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 
 import paged_ref as ref
-from test_gpu_paged import RANGE, TYPES, Meta, Pool, attend, check_attention, check_on_gpu, dev, host, make, tt
+from test_gpu_paged import RANGE, TYPES, Meta, Pool, attend, check_attention, check_on_gpu, dev, host, make, row_bound, tables, tt
 from test_gpu_paged import torch as torch  # the fixture
 
 pytestmark = pytest.mark.gpu
@@ -287,3 +287,167 @@ def test_a_score_of_minus_infinity_has_no_weight(pkg, torch, t, kv, new, total, 
         assert np.isnan(got[last]).all() and np.isnan(gl[last]).all()
         other = slice(b.new[0], rows)
         assert np.all(np.abs(got - out)[other] <= bound[other])
+
+
+# ---------------------------------------------------------------- append: what is left alone
+def append_call(pkg, torch, b, x, pool, m, hq, hk, rope=None, t="f32"):
+    """x [rows][hq + 2 hk][d]; q goes through to rows of -7. Returns q's rows and the status."""
+    d = x.shape[2]
+    buf = dev(torch, x.reshape(b.rows, -1)).to(tt(torch, t))
+    qo, st = torch.full((b.rows, hq * d), -7.0, dtype=buf.dtype, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda")
+    at, e, w = buf.data_ptr(), buf.element_size(), buf.shape[1]
+    kw = {} if rope is None else dict(cos_ptr=rope[0].data_ptr(), sin_ptr=rope[1].data_ptr(), rope_rows=rope[0].shape[0],
+                                      rope_half_dim=rope[0].shape[1])
+    pkg.engine.paged_append(at + hq * d * e, at + (hq + hk) * d * e, b.rows, hk, d, **pool.args(), **m.kw, q_ptr=at,
+                            q_out_ptr=qo.data_ptr(), q_heads=hq, dtype=t, q_stride=w, k_stride=w, v_stride=w,
+                            status_ptr=st.data_ptr(), **kw)
+    torch.cuda.synchronize()
+    return host(qo).reshape(b.rows, hq, d), int(st.item())
+
+
+@pytest.mark.parametrize("start,kept", [
+    ([-2, 1, 2, 3, 4, 5, 6, 7, 100], [1, 2, 3, 4, 5, 6]),      # the first and the last range lie outside the rows
+    ([0, 1, 2, 3, 4, 5, 6, 7, 9], [0, 1, 2, 3, 4, 5, 6]),
+    ([3, 4, 5, 5, 5, 5, 5, 6, 7], [3, 4, 5, 6]),               # rows before the first and behind the last sequence
+    ([-2, 1, 2, 9, 1, 0, 6, 7, 100], None)])                   # in no order: nothing outside the sequences' places
+def test_append_of_bad_row_ranges_leaves_the_pool_alone(pkg, torch, start, kept):
+    rng = np.random.default_rng(3)
+    b = ref.Batch(rng, [1] * 8, [4, 3, 4, 2, 1, 4, 4, 4], 4, wide=2)
+    x = rng.standard_normal((8, 4, 64)).astype(np.float32)
+    before = [rng.standard_normal((b.pages, 4, 1, 64)).astype(np.float32) for _ in range(2)]
+    pool, m = Pool(torch, "f32", b, 1, 64, "slot", before), Meta(torch, b)
+    m.start.copy_(dev(torch, np.array(start, np.int32)))
+    got, st = append_call(pkg, torch, b, x, pool, m, 2, 1)
+    assert st == (RANGE if start[0] < 0 or start[-1] > 8 else 0)
+    if kept is None:  # every place that differs is that of a sequence's newest positions
+        own = np.zeros(before[0].shape[:2], bool)
+        for s in range(8):
+            for p in range(b.total[s]):
+                own[b.place(s, p)] = True
+        assert all(np.array_equal(u[~own], w[~own]) for u, w in zip(pool.values(), before))
+        return
+    want = [z.copy() for z in before]
+    for row in kept:
+        s = max(i for i in range(8) if start[i] <= row)
+        for z, h in zip(want, (2, 3)):
+            z[b.place(s, b.total[s] - 1)] = x[row, h]
+    assert all(np.array_equal(u, w) for u, w in zip(pool.values(), want))
+    gone = [r for r in range(8) if r not in kept]
+    assert np.array_equal(got[kept], x[kept, :2]) and np.all(got[gone] == -7.0)
+
+
+@pytest.mark.parametrize("t,kv", TYPES)
+def test_append_behind_the_rotation_tables(pkg, torch, t, kv):
+    """Positions that the tables do not reach: k, v and q of those rows stay as they were."""
+    rng = np.random.default_rng(4)
+    b = ref.Batch(rng, [5, 1, 2], [12, 10, 3], 4)
+    top, hq, hk, d = 10, 3, 2, 64
+    x = ref.round_to(rng.standard_normal((b.rows, hq + 2 * hk, d)), t)
+    before = [ref.round_to(rng.standard_normal((b.pages, 4, hk, d)), kv) for _ in range(2)]
+    cos, sin = tables(rng, top, 32)
+    pool, m = Pool(torch, kv, b, hk, d, "head", before), Meta(torch, b)
+    got, st = append_call(pkg, torch, b, x, pool, m, hq, hk, rope=(dev(torch, cos), dev(torch, sin)), t=t)
+    assert st == RANGE
+    want, near = [z.copy() for z in before], np.zeros_like(before[0])
+    for s in range(b.seqs):
+        for i in range(b.new[s]):
+            p, row = b.total[s] - b.new[s] + i, b.start[s] + i
+            if p >= top:
+                assert np.all(got[row] == -7.0)
+                continue
+            val, mag = ref.norm_rope(x[row:row + 1, :hq + hk], None, 0, cos[p:p + 1], sin[p:p + 1])
+            assert np.all(np.abs(got[row] - val[0, :hq]) <= row_bound(val, mag, t)[0, :hq])
+            at = b.place(s, p)
+            want[0][at], near[at] = val[0, hq:], row_bound(val, mag, kv)[0, hq:]
+            want[1][at] = ref.round_to(x[row, hq + hk:], kv)
+    kp, vp = pool.values()
+    assert np.array_equal(vp, want[1]) and np.all(np.abs(kp - want[0]) <= near)
+
+
+@pytest.mark.parametrize("t,kv", TYPES)
+def test_append_to_a_page_that_does_not_exist_turns_q(pkg, torch, t, kv):
+    rng = np.random.default_rng(5)
+    b = ref.Batch(rng, [2, 1], [6, 3], 4)
+    x = ref.round_to(rng.standard_normal((b.rows, 3, 64)), t)
+    before = [ref.round_to(rng.standard_normal((b.pages, 4, 1, 64)), kv) for _ in range(2)]
+    want = [z.copy() for z in before]
+    for z, h in zip(want, (1, 2)):
+        z[b.place(1, 2)] = ref.round_to(x[2, h], kv)
+    b.table[0, 1] = b.pages
+    pool, m = Pool(torch, kv, b, 1, 64, "slot", before), Meta(torch, b)
+    got, st = append_call(pkg, torch, b, x, pool, m, 1, 1, t=t)
+    assert st == RANGE and np.array_equal(got[:, 0], x[:, 0])
+    assert all(np.array_equal(u, w) for u, w in zip(pool.values(), want))
+
+
+# ---------------------------------------------------------------- strides
+@pytest.mark.parametrize("t,kv", TYPES)
+@pytest.mark.parametrize("page,layout,d", [(8, "slot", 64), (16, "head", 128), (16, "slot", 128), (64, "head", 64), (128, "slot", 128),
+                                           (128, "head", 64), (256, "head", 128)])
+@pytest.mark.parametrize("gap", [8, 64])
+@pytest.mark.parametrize("new,total,window", [([200, 90], [700, 333], 0), ([130, 1, 3], [130, 300, 515], 150)])
+def test_pages_with_gaps(pkg, torch, t, kv, page, layout, d, gap, new, total, window):
+    """NaN between the rows of the pages (TMA boxes of padded slots, heads and pages)."""
+    rng = np.random.default_rng(page + gap)
+    b, q, pages, pool = make(torch, rng, t, kv, new, total, page, layout, 4, 2, d, gap=gap)
+    got, gl, st = attend(pkg, torch, b, q, pool, t, window=window, pad=8, qpad=24)
+    assert st == 0
+    for z, p in zip(pool.t, pages):
+        p = p if layout == "slot" else p.transpose(0, 2, 1, 3)
+        z[..., :d] = dev(torch, np.nan_to_num(p, nan=0.0, posinf=0.0)).to(z.dtype)  # stale slots, for the 64-bit form
+    check_on_gpu(torch, b, got, gl, q, pool, t, kv, window)
+
+
+@pytest.mark.parametrize("t,kv", TYPES)
+@pytest.mark.parametrize("n", [1, 150])
+def test_k_and_v_interleaved_in_one_pool(pkg, torch, t, kv, n):
+    """[page][K, V][slot][head][d], pages twice as far apart as they are long."""
+    page, hk, d = 16, 2, 64
+    rng = np.random.default_rng(n)
+    b = ref.Batch(rng, [n, n], [400, 220], page)
+    both = torch.randn(b.pages, 2, page, hk, d, device="cuda").to(tt(torch, kv))
+    pool = Pool.__new__(Pool)
+    pool.torch, pool.kv, pool.b, pool.hk, pool.d, pool.layout = torch, kv, b, hk, d, "slot"
+    pool.t, pool.strides = [both[:, 0], both[:, 1]], (2 * page * hk * d, d, hk * d)
+    q = ref.round_to(rng.standard_normal((b.rows, 6, d)), t)
+    got, gl, st = attend(pkg, torch, b, q, pool, t)
+    assert st == 0
+    check_on_gpu(torch, b, got, gl, q, pool, t, kv)
+
+
+# ---------------------------------------------------------------- log-sum-exp
+def lse_bound(wl, size, longest, dim):
+    """lse is made of unrounded f32 weights: an error ds of each score (attention_bounds) with the
+    exponential's own, the f32 sum over the positions (2^-23 each), log2 (2^-22) and its two
+    roundings with the sum's logarithm and the maximum, up to |lse| + 16 (2^-23 of it)."""
+    ds = (dim * 2.0**-23 + 2.0**-21) * size + 2.0**-20
+    return ds + longest * 2.0**-23 + 2.0**-22 + 2.0**-23 * (np.abs(wl) + 16)
+
+
+@pytest.mark.parametrize("t,kv", TYPES)
+@pytest.mark.parametrize("new,total,window", [([1, 1, 1], [2, 700, 63], 0), ([3, 2], [300, 40], 25), ([90, 40], [300, 41], 0), ([140], [420], 64)])
+def test_log_sum_exp_counts_unrounded_weights(pkg, torch, t, kv, new, total, window):
+    rng = np.random.default_rng(sum(total))
+    b, q, pages, pool = make(torch, rng, t, kv, new, total, 16, "head", 4, 2, 64, extra=0)
+    got, gl, st = attend(pkg, torch, b, q, pool, t, window=window)
+    _, wl, _, size = ref.attention(b, q, *pages, 0.125, window)
+    assert st == 0 and np.all(np.abs(gl - wl) <= lse_bound(wl, size, max(total), 64))
+
+
+@pytest.mark.parametrize("t,kv", TYPES)
+@pytest.mark.parametrize("n", [1, 100])
+def test_log_sum_exp_of_equal_scores(pkg, torch, t, kv, n):
+    """Weights that a 16-bit type cannot hold: with scores of 0 and one of ln 1.0039 (q = 0 but
+    for one element), the sum is known, and a rounded weight would show."""
+    rng = np.random.default_rng(1)
+    b, q, pages, pool = make(torch, rng, t, kv, [n], [260], 16, "slot", 2, 1, 64, extra=0)
+    q[:] = 0.0
+    q[:, :, 0] = 1.0
+    for p in range(260):
+        pages[0][b.place(0, p)] = 0.0
+        pages[0][b.place(0, p) + (0, 0)] = ref.round_to(0.0039 * (p % 7), kv)
+    pool = Pool(torch, kv, b, 1, 64, "slot", pages)
+    got, gl, st = attend(pkg, torch, b, q, pool, t, scale=1.0)
+    _, wl, _, size = ref.attention(b, q, *pages, 1.0, 0)
+    # one product per score, exact: the scores' error is that of the exponential alone
+    assert st == 0 and np.all(np.abs(gl - wl) <= 2.0**-20 + 260 * 2.0**-23 + 2.0**-22 + 2.0**-23 * (np.abs(wl) + 16))
