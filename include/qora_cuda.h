@@ -347,10 +347,11 @@ qora_status qora_q4_lm_head(const float* d_x, const uint8_t* d_packed,
  * Types. Rows f32 with pages f32 or f16, rows and pages f16, rows and pages bf16. Sums,
  * norms and softmax statistics are f32 throughout; a value is rounded once, to nearest
  * even, where it is written (binary16 beyond +-65504 becomes infinite). What the tensor
- * cores multiply: 16-bit values as they are, the softmax weights rounded to the rows' 16
- * bits (half a step of each weight); f32 values, and their weights, as two halves of 22
- * bits together. Before the division by the sum of the weights these are up to 2^15 times
- * their final size: |v| from 2^90 on may overflow.
+ * cores multiply: 16-bit values as they are, their softmax weights rounded to the rows' 16
+ * bits (half a step of each weight; for sequences of few new rows in two parts of 22 bits
+ * together, 16 of bf16); f32 values, and their weights, as two halves of 22 bits together.
+ * Before the division by the sum of the weights these are up to 2^15 times their final size:
+ * |v| from 2^90 on may overflow.
  *
  * What the host cannot see is checked on the device: a sequence whose rows lie outside
  * [0, rows) or whose length does not fit its table row, a position behind the rotation

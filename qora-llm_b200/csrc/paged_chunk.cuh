@@ -35,7 +35,10 @@
 // power of two: q by row, K and V by tile (largest value in [2^13, 2^14)). The weights are
 // split too. Upper x upper, lower x upper and upper x lower are multiplied: two products
 // instead of one for an f16 cache, three for an f32 cache. The scale of K goes into the
-// scores' scale. V's scales differ from tile to tile; the numerators count in the smallest
+// scores' scale. 16-bit rows' weights are rounded to the rows' type, which adds about as much
+// error as the rounding of the result: a lower part as well would take 8,192 binary16 rows from
+// 258 to 351 us (rms error 2.14e-5; 1.64e-5 with it), mixed bf16 chunks from 98 to 126 us. V's
+// scales differ from tile to tile; the numerators count in the smallest
 // so far (the largest values) and the weights of other tiles are scaled down to it.
 //
 // The running maximum is raised only when it grows by more than 2^kSlack: then the

@@ -451,3 +451,25 @@ def test_log_sum_exp_of_equal_scores(pkg, torch, t, kv, n):
     _, wl, _, size = ref.attention(b, q, *pages, 1.0, 0)
     # one product per score, exact: the scores' error is that of the exponential alone
     assert st == 0 and np.all(np.abs(gl - wl) <= 2.0**-20 + 260 * 2.0**-23 + 2.0**-22 + 2.0**-23 * (np.abs(wl) + 16))
+
+
+# ---------------------------------------------------------------- the weights' bits
+@pytest.mark.parametrize("t,kv", TYPES)
+@pytest.mark.parametrize("new,total", [([1, 1, 1], [2, 90, 40]), ([2, 1], [60, 7]), ([30, 40], [30, 60])])
+def test_weights_are_as_exact_as_they_are_said_to_be(pkg, torch, t, kv, new, total):
+    """q = 0 but for one element, so that the scores are exact: what is left is the weights' own
+    error, 22 bits (bf16: 16) for few rows and f32 rows, half a step of the type for chunks."""
+    rng = np.random.default_rng(3)
+    b, q, pages, _ = make(torch, rng, t, kv, new, total, 16, "slot", 2, 1, 64, extra=0)
+    q[:, :, 1:] = 0.0
+    pages[0] = np.nan_to_num(pages[0], nan=0.0, posinf=0.0)
+    pages[0][..., 1:] = 0.0
+    got, gl, st = attend(pkg, torch, b, q, Pool(torch, kv, b, 1, 64, "slot", pages), t, scale=1.0)
+    out, _, mass, size = ref.attention(b, q, *pages, 1.0, 0)
+    weight = 2.0**-21 if t == "f32" else {"f16": 2.0**-21, "bf16": 2.0**-16}[t] if max(new) <= 2 else ref.HALF_STEP[t]
+    ds = 2.0**-20 + 2.0**-22 * size  # an exact product, its scaling by log2(e), the exponential
+    if t == "f32":
+        ds = ds + 2.0**-21 * size
+    rel = 2 * ds + weight + 2 * max(total) * 2.0**-23
+    bound = rel[..., None] * mass * 1.01 + ref.HALF_STEP[t] * np.abs(out) * 1.01 + 2 * ref.TINY[t]
+    assert st == 0 and np.all(np.abs(got - out) <= bound)
