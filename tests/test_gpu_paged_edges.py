@@ -473,3 +473,28 @@ def test_weights_are_as_exact_as_they_are_said_to_be(pkg, torch, t, kv, new, tot
     rel = 2 * ds + weight + 2 * max(total) * 2.0**-23
     bound = rel[..., None] * mass * 1.01 + ref.HALF_STEP[t] * np.abs(out) * 1.01 + 2 * ref.TINY[t]
     assert st == 0 and np.all(np.abs(got - out) <= bound)
+
+
+@pytest.mark.parametrize("t,kv", TYPES)
+@pytest.mark.parametrize("n", [1, 70])
+@pytest.mark.parametrize("gap", [4, 9, 14, 18])
+def test_small_weights_beside_a_large_one(pkg, torch, t, kv, n, gap):
+    """One position whose score lies `gap` above all others, with a value of 0: the result is made
+    of small weights alone. They have their relative error, or 2^-31 of the largest weight."""
+    rng = np.random.default_rng(gap)
+    L = 300
+    b, q, pages, _ = make(torch, rng, t, kv, [n], [L], 16, "slot", 2, 1, 64, extra=0)
+    q[:] = 0.0
+    q[:, :, 0] = 1.0
+    pages[0] = np.zeros_like(pages[0])
+    pages[1] = ref.round_to(np.abs(np.nan_to_num(pages[1], nan=0.0, posinf=0.0)) + 1.0, kv)
+    pg, sl = b.place(0, 20)
+    pages[0][pg, sl, 0, 0], pages[1][pg, sl] = gap, 0.0
+    got, gl, st = attend(pkg, torch, b, q, Pool(torch, kv, b, 1, 64, "slot", pages), t, scale=1.0)
+    out, _, mass, size = ref.attention(b, q, *pages, 1.0, 0)
+    weight = {"f32": 2.0**-21, "f16": 2.0**-21 if n == 1 else 2.0**-11, "bf16": 2.0**-16 if n == 1 else 2.0**-8}[t]
+    ds = 2.0**-20 + 2.0**-21 * size  # exact products, their scaling by log2(e), the exponential
+    rel = 2 * ds + weight + 2 * L * 2.0**-23
+    floor = 0.0 if t == "bf16" else L * 2.0**-31 * np.abs(pages[1]).max()
+    bound = rel[..., None] * mass * 1.01 + floor + ref.HALF_STEP[t] * np.abs(out) * 1.01 + 2 * ref.TINY[t]
+    assert st == 0 and np.all(np.abs(got - out) <= bound)
