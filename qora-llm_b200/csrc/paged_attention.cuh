@@ -29,6 +29,9 @@ struct AttnArgs {
   unsigned* status;
 };
 
+// token of packed row r (< 128) of a tile: r / group
+QORA_DEV int token_of(const AttnArgs& a, int r) { return (r * a.group_inv) >> 16; }
+
 // The first position that a row at position p attends to. p may be negative (more new rows
 // than positions), the window up to 2^31 - 1.
 QORA_DEV int first_seen(const AttnArgs& a, int p) { return a.window > 0 ? max(0, max(p, -1) + 1 - a.window) : 0; }

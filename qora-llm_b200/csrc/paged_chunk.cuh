@@ -234,9 +234,6 @@ struct ItemRange {
   int part, parts;                        // partial slot, or -1: the item is whole; the item's parts
 };
 
-// token of packed row r (< 128) of a block: r / group
-QORA_DEV int row_token(const AttnArgs& a, int r) { return (r * a.group_inv) >> 16; }
-
 // The sequences' row tiles as a warp holds them: a lane sums a run of neighbouring sequences.
 // Rows that no two sequences share make at most 2^24 / tokens + 2^20 tiles, below kManyTiles; a
 // lane that counts more (overlapping ranges) stays there, so that the warp's sum cannot wrap
@@ -823,7 +820,7 @@ __global__ void __launch_bounds__(ChunkCfg<T, C, D>::kThreads, 1)
     const int x = warp >> 2, r0 = (warp & 3) * 32, r = r0 + lane;
     const uint32_t ts = tmem + x * 128 + ((uint32_t)r0 << 16), to = tmem + 256 + x * D + ((uint32_t)r0 << 16);
     const float scale2 = a.scale * kLog2e;
-    const int rtok = row_token(a, r);  // token of the thread's row within the block
+    const int rtok = token_of(a, r);  // token of the thread's row within the block
     uint32_t seen = 0, o_turn = 0, tiles = 0;
     bool ok = true;  // the same for the whole warp
     auto wait_all = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; };
@@ -852,7 +849,7 @@ __global__ void __launch_bounds__(ChunkCfg<T, C, D>::kThreads, 1)
           int ups[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const int rr = r0 + 8 * i + (lane >> 2), tok = row_token(a, rr);
+            const int rr = r0 + 8 * i + (lane >> 2), tok = token_of(a, rr);
             const bool there = tok < toks;
             const float* src = reinterpret_cast<const float*>(a.q) + (there ? (row0 + tok) * a.q_stride + (it.head * a.group + rr - tok * a.group) * D : 0) + sub * 4;
             float4 y[kF4];
@@ -1062,7 +1059,7 @@ __global__ void __launch_bounds__(ChunkCfg<T, C, D>::kThreads, 1)
         const float mula = __shfl_sync(0xffffffffu, mul, ra), mulb = __shfl_sync(0xffffffffu, mul, ra + 8);
         const bool la = (live_rows >> ra) & 1, lb = (live_rows >> (ra + 8)) & 1;
         auto out_row = [&](int rr) {  // output of packed row rr of the block
-          const int tok = row_token(a, rr);
+          const int tok = token_of(a, rr);
           return static_cast<T*>(a.out) + (row0 + tok) * a.out_stride + (it.head * a.group + rr - tok * a.group) * D;
         };
         T* const oa = out_row(r0 + ra);
@@ -1169,7 +1166,7 @@ __global__ void __launch_bounds__(ChunkCfg<T, C, D>::kThreads, 1)
       const T* q[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int tok = row_token(a, first_row + i);
+        const int tok = token_of(a, first_row + i);
         const bool live = tok < toks;
         const long long row = row0 + (live ? tok : 0);
         const int h = it.head * a.group + (live ? first_row + i - tok * a.group : 0);
@@ -1186,8 +1183,8 @@ __global__ void __launch_bounds__(ChunkCfg<T, C, D>::kThreads, 1)
       for (int i = 0; i < 4; ++i) {
         const float mi = __shfl_sync(0xffffffffu, m, 8 * i), li = __shfl_sync(0xffffffffu, l, 8 * i);
         if (at[i] < 0) continue;
-        const int h = it.head * a.group + first_row + i - row_token(a, first_row + i) * a.group;
-        const long long row = row0 + row_token(a, first_row + i);
+        const int h = it.head * a.group + first_row + i - token_of(a, first_row + i) * a.group;
+        const long long row = row0 + token_of(a, first_row + i);
         const size_t part_row = (size_t)max(it.part, 0) * 256 + x * 128 + first_row + i;
         const float inv = li == 0.0f ? 0.0f : __fdiv_rn(1.0f, li);
 #pragma unroll
@@ -1217,7 +1214,7 @@ __global__ void __launch_bounds__(256) chunk_join_kernel(const AttnArgs a, void*
   const int4 rec = chunk_rec(work)[blockIdx.x];  // (first row, tokens, kv head, slots and parts)
   const int splits = rec.w & 0xffff;
   const int lane = threadIdx.x & 31, rr = blockIdx.y * 8 + (threadIdx.x >> 5), x = rr >> 7, r = rr & 127;
-  const int block_toks = 128 / a.group, rtok = row_token(a, r), tok = x * block_toks + rtok;
+  const int block_toks = 128 / a.group, rtok = token_of(a, r), tok = x * block_toks + rtok;
   if (rtok >= block_toks || tok >= rec.y) return;
   const size_t first = (size_t)blockIdx.x * (rec.w >> 16) * 256 + rr;
   float mm = -INFINITY;

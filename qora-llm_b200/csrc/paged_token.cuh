@@ -95,9 +95,6 @@ QORA_DEV void mma_tf32(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint3
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// token of packed row r (< 16) of a tile: r / group
-QORA_DEV int token_of(const AttnArgs& a, int r) { return (r * a.group_inv) >> 16; }
-
 QORA_DEV uint32_t pack2(float a, float b, __half) {
   const __half2 h = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&h);
