@@ -498,3 +498,62 @@ def test_small_weights_beside_a_large_one(pkg, torch, t, kv, n, gap):
     floor = 0.0 if t == "bf16" else L * 2.0**-31 * np.abs(pages[1]).max()
     bound = rel[..., None] * mass * 1.01 + floor + ref.HALF_STEP[t] * np.abs(out) * 1.01 + 2 * ref.TINY[t]
     assert st == 0 and np.all(np.abs(got - out) <= bound)
+
+
+# ---------------------------------------------------------------- heads and graphs
+@pytest.mark.parametrize("t,kv", TYPES)
+@pytest.mark.parametrize("hq,hk,d", [(128, 1, 64), (100, 1, 64), (7, 1, 128), (10, 2, 64), (33, 3, 64), (36, 2, 128)])
+@pytest.mark.parametrize("new,total,window", [([1, 1], [90, 7], 0), ([5, 2], [40, 70], 30), ([19], [140], 0)])
+def test_any_number_of_heads_per_kv_head(pkg, torch, t, kv, hq, hk, d, new, total, window):
+    rng = np.random.default_rng(hq)
+    b, q, pages, pool = make(torch, rng, t, kv, new, total, 16, "slot", hq, hk, d)
+    got, gl, st = attend(pkg, torch, b, q, pool, t, window=window)
+    assert st == 0
+    check_attention(b, got, gl, q, pages, t, kv, d ** -0.5, window)
+
+
+@pytest.mark.parametrize("t,kv", TYPES)
+def test_a_captured_batch_of_tokens_and_chunks_grows(pkg, torch, t, kv):
+    """Single tokens and chunks in one captured call (both kernels and their joins), replayed with
+    other lengths, other row ranges and another table."""
+    hq, hk, d, page, window = 8, 4, 64, 16, 900
+    rng = np.random.default_rng(16)
+    rounds = [[1] * 40 + [150, 90], [1] * 39 + [33, 1, 207], [0, 2] * 20 + [200, 0]]
+    totals = [[n + int(rng.integers(0, 1000)) for n in new] for new in rounds]
+    rows, wide, seqs = 280, 80, 42
+    pages = 3000
+    g = torch.Generator(device="cuda").manual_seed(3)
+    first = ref.Batch(np.random.default_rng(0), rounds[0], totals[0], page, wide=wide)
+    first.pages = pages
+    pool = Pool(torch, kv, first, hk, d, "slot")
+    for z in pool.t:
+        z.copy_(torch.randn(z.shape, generator=g, device="cuda"))
+    m = Meta(torch, first)
+    dq = torch.zeros(rows, hq * d, dtype=tt(torch, t), device="cuda")
+    out, lse = torch.empty_like(dq), torch.empty(rows, hq, device="cuda")
+    work = torch.empty(pkg.engine.PAGED_WORK_BYTES, dtype=torch.uint8, device="cuda")
+    st = torch.zeros(1, dtype=torch.int32, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        pkg.engine.paged_attention(dq.data_ptr(), out.data_ptr(), rows, hq, hk, d, **pool.args(), **m.kw, max_q=207,
+                                   work_ptr=work.data_ptr(), window=window, lse_ptr=lse.data_ptr(), dtype=t,
+                                   status_ptr=st.data_ptr(), stream=torch.cuda.current_stream())
+    for new, total in zip(rounds, totals):
+        b = ref.Batch(rng, new, total, page, wide=wide)
+        table = rng.integers(0, pages, seqs * wide).astype(np.int32)  # pages may be shared
+        b.table = table.reshape(seqs, wide)
+        q = ref.round_to(rng.standard_normal((rows, hq, d)) * 1.5, t)
+        dq.copy_(dev(torch, q.reshape(rows, -1)))
+        for x, y in ((m.start, b.start), (m.len, b.len), (m.table, b.table)):
+            x.copy_(dev(torch, y))
+        out.fill_(-7.0)
+        work.fill_(255)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert int(st.item()) == 0
+        got = host(out).reshape(rows, hq, d)
+        assert np.all(got[b.start[-1]:] == -7.0)
+        live = [s for s in range(seqs) if new[s]]  # the 64-bit form is of sequences with rows
+        b.seqs, b.new, b.total = len(live), [new[s] for s in live], [total[s] for s in live]
+        b.start, b.table = np.append(b.start[live], b.start[-1]), b.table[live]
+        check_on_gpu(torch, b, got, host(lse), q, pool, t, kv, window)
