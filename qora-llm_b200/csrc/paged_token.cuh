@@ -20,8 +20,10 @@
 // cp.async stages, running maximum and sum; there is no barrier until the segment's end.
 // Weights of 16-bit rows are multiplied in two parts too, upper and lower (22 bits, 16 of bf16):
 // 128 binary16 tokens are then as close to the exact result as rounding lets them be (rms
-// error 1.36e-5; weights rounded to binary16: 1.85e-5), in 177 us instead of 176 us (64 windowed
-// tokens over 1,000 positions: 38 to 39 us instead of 35 to 37 us).
+// error 1.36e-5; weights rounded to binary16: 1.85e-5). Up to 8 packed rows leave the
+// instruction's rows 8-15 for the lower parts (189 us instead of 188 us, consecutive calls on
+// changing inputs; as instructions of their own 203 us); more rows take a second instruction
+// (64 sequences of 1 to 4 rows over 4,000 positions: 96 us instead of 94 us).
 // The maximum is only raised (and the numerators rescaled) when it grows by more than
 // 2^kSlack, so weights stay below 2^(kShift + kSlack) <= 2^15, within binary16.
 //
@@ -280,6 +282,7 @@ __global__ void __launch_bounds__(32 * TokenCfg<T, C, D>::kWarps, 1) token_kerne
       continue;
     }
     const int nrows = sw.n * a.group;
+    const bool spare = !kHalves && nrows <= 8;  // the instruction's rows 8-15 take the weights' lower parts
     const int p0 = sw.len - sw.n;
     const int* table = a.batch.table + (long long)seq * a.batch.table_stride;
     const C* kbase = static_cast<const C*>(a.k_pages) + head * a.pg.head_stride;
@@ -543,7 +546,7 @@ __global__ void __launch_bounds__(32 * TokenCfg<T, C, D>::kWarps, 1) token_kerne
             m[r] = mn;
             l[r] *= f[r];
           }
-          if (kHalves) f[1] = f[0];
+          if (kHalves || spare) f[1] = f[0];
 #pragma unroll
           for (int x = 0; x < kO; ++x) {
             o[x][0] *= f[0];
@@ -582,28 +585,17 @@ __global__ void __launch_bounds__(32 * TokenCfg<T, C, D>::kWarps, 1) token_kerne
             }
           }
         } else {
-          uint32_t pa[4], pl[4];
-          if constexpr (kHalves) {
-#pragma unroll
-            for (int n = 0; n < 2; ++n) {
-              const uint32_t hi = pack2(s[n][0], s[n][1], __half());
-              const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&hi));
-              pa[2 * n] = hi;
-              pa[2 * n + 1] = pack2(s[n][0] - h.x, s[n][1] - h.y, __half());
-            }
-          } else {
-#pragma unroll
-            for (int n = 0; n < 2; ++n) {
-#pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                const uint32_t hi = pack2(s[n][2 * h], s[n][2 * h + 1], C());
-                const C* e = reinterpret_cast<const C*>(&hi);
-                pa[2 * n + h] = hi;
-                pl[2 * n + h] = pack2(s[n][2 * h] - to_f32(e[0]), s[n][2 * h + 1] - to_f32(e[1]), C());
-              }
-            }
-          }
           const int mi = lane >> 3, row = (mi & 1) * 8 + (lane & 7);
+          auto lower = [&](uint32_t hi, float x, float y) {  // what the upper parts `hi` of two weights leave
+            const C* e = reinterpret_cast<const C*>(&hi);
+            return pack2(x - to_f32(e[0]), y - to_f32(e[1]), C());
+          };
+          uint32_t pa[4];
+#pragma unroll
+          for (int n = 0; n < 2; ++n) {
+            pa[2 * n] = pack2(s[n][0], s[n][1], C());
+            pa[2 * n + 1] = kHalves || spare ? lower(pa[2 * n], s[n][0], s[n][1]) : pack2(s[n][2], s[n][3], C());
+          }
 #pragma unroll
           for (int d = 0; d < D / 16; ++d) {
             uint32_t b[4];
@@ -618,8 +610,20 @@ __global__ void __launch_bounds__(32 * TokenCfg<T, C, D>::kWarps, 1) token_kerne
                 o[2 * d + 1][x] += acc[1][x];
               }
             } else {
-              mma16(o[2 * d], pl, b[0], b[1], C());
-              mma16(o[2 * d + 1], pl, b[2], b[3], C());
+              mma16(o[2 * d], pa, b[0], b[1], C());
+              mma16(o[2 * d + 1], pa, b[2], b[3], C());
+            }
+          }
+          if (!kHalves && !spare) {
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+              pa[2 * n] = lower(pa[2 * n], s[n][0], s[n][1]);
+              pa[2 * n + 1] = lower(pa[2 * n + 1], s[n][2], s[n][3]);
+            }
+#pragma unroll
+            for (int d = 0; d < D / 16; ++d) {
+              uint32_t b[4];
+              ldsm4_t(b, sv + Cfg::v_at(row, 2 * d + (mi >> 1)));
               mma16(o[2 * d], pa, b[0], b[1], C());
               mma16(o[2 * d + 1], pa, b[2], b[3], C());
             }
@@ -673,6 +677,8 @@ __global__ void __launch_bounds__(32 * TokenCfg<T, C, D>::kWarps, 1) token_kerne
 #pragma unroll
         for (int x = 0; x < kO; ++x) {
           if constexpr (kHalves) {
+            *reinterpret_cast<float2*>(dst + 8 * x + 2 * t) = make_float2(o[x][0] + o[x][2], o[x][1] + o[x][3]);
+          } else if (spare) {
             *reinterpret_cast<float2*>(dst + 8 * x + 2 * t) = make_float2(o[x][0] + o[x][2], o[x][1] + o[x][3]);
           } else {
             *reinterpret_cast<float2*>(dst + 8 * x + 2 * t) = make_float2(o[x][0], o[x][1]);
