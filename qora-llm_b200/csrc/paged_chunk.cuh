@@ -9,10 +9,10 @@
 // leave half of the CTAs idle, the positions of each are split evenly and chunk_join_kernel
 // adds the parts in order; a part has one tile at least (8 short prompts in 18.5 us, with
 // empty parts 20.6 us; parts of two tiles or more: 14 prompts over 500 positions in 23.7 us
-// instead of 20.6 us). Items are taken from the last rows (the longest runs of positions)
-// on, in alternating direction, so the CTAs end together: 8,192 rows in 264 us. Equal shares
-// of one line of tiles, as the token kernel has, cost more in items begun twice than they
-// even out (314 us; 240 items of a mixed batch in 126 us instead of 99 us).
+// instead of 20.6 us). Items are taken from the last rows (the longest runs of positions
+// of one prompt) on, in alternating direction. Equal shares of one line of tiles, as the token
+// kernel has, cost more in items begun twice than they even out (8,192 rows in 314 us instead
+// of 264 us; 240 items of a mixed batch in 126 us instead of 99 us).
 //
 // Roles (one CTA per SM):
 //   warps 0-3, 4-7   softmax of block 0, 1: a thread owns a row, keeps its scores in
@@ -38,8 +38,8 @@
 // scores' scale. 16-bit rows' weights are rounded to the rows' type, which adds about as much
 // error as the rounding of the result: a lower part as well would take 8,192 binary16 rows from
 // 258 to 351 us (rms error 2.14e-5; 1.64e-5 with it), mixed bf16 chunks from 98 to 126 us. V's
-// scales differ from tile to tile; the numerators count in the smallest
-// so far (the largest values) and the weights of other tiles are scaled down to it.
+// scales differ from tile to tile; the numerators count in the smallest so far (the largest
+// values) and the weights of other tiles are scaled down to it.
 //
 // The running maximum is raised only when it grows by more than 2^kSlack: then the
 // numerators in TMEM are scaled, which is rare after the first tiles. Masked scores become
@@ -47,14 +47,15 @@
 // infinite value of V, or a row whose own scores are) are computed again in f32 when the CTA's
 // roles have ended (rows_attend). So are rows of an f32 cache that meet a tile of K or V whose
 // rows differ by more than 2^14 in size, a tile of V 2^12 below the largest before it, or
-// growth of V by more than 2^60. This is for correctness alone, and 15 to 70 times as slow:
-// where every row is concerned, 1,021 f32 rows take 0.85 ms instead of 56 us, 512 f32 rows
-// over 8,192 binary16 positions 4.4 ms, 2,048 binary16 rows 4.2 ms instead of 42 us (one row
-// and one position at a time, between the tiles, took 10, 41 and 40 ms).
+// growth of V by more than 2^60. This is for correctness alone, and 15 to 90 times as slow:
+// where every row is concerned, 1,021 f32 rows take 0.84 ms instead of 58 us, 512 f32 rows
+// over 8,192 binary16 positions 4.4 ms instead of 86 us, 2,048 binary16 rows 4.2 ms instead of
+// 47 us (one row and one position at a time, between the tiles, took 10, 41 and 40 ms).
 //
-// Measured, 16 query heads over 4 kv heads of 128: a prompt of 8,192 binary16 rows in 264 to
-// 272 us = 1.01 to 1.04 PFLOP/s of 275 GFLOP; 512 f32 rows over 8,192 binary16 positions in
-// 83 us; a prompt of 1,021 rows, all f32, in 54 us.
+// Measured, 16 query heads over 4 kv heads of 128, short runs of the same call (in brackets:
+// consecutive calls on changing inputs, under the power cap): a prompt of 8,192 binary16 rows,
+// 275 GFLOP, in 257 to 273 us = 1.01 to 1.07 PFLOP/s (301 us); 512 f32 rows over 8,192 binary16 positions in
+// 83 us (89 us); a prompt of 1,021 rows, all f32, in 56 us (61 us).
 #pragma once
 
 #include <cuda.h>

@@ -260,16 +260,17 @@ qora_status launch_chunk(const paged::AttnArgs& a, void* work, cudaStream_t s) {
   return QORA_OK;
 }
 
-// Sequences with at most `few` new rows are the token kernel's, which reads their pages as
-// fast as memory gives them (64 sequences of 1 to 4 rows over 4,000 positions: 94 us with
-// f16, 184 us with f32 caches; the chunk kernel: 147 us and 540 us for 1 to 5 rows); longer
-// ones the chunk kernel's. Both run where short sequences are likely (the longest is far
-// longer than the mean, or the others are short on average; the host does not know) and
-// are more than the chunk kernel would have in one turn of its CTAs, half of that with an
-// f32 cache: 60 tokens over 4,000 positions with 4 chunks of 512 rows over 2,000 take 147 us
-// with f16, 371 us with f32 caches (the chunk kernel alone: 196 and 711 us), but 31 tokens
-// over 2,000 with a chunk of 256 rows 60 us with f16 caches (alone: 44 us; f32: 98 and 141
-// us). A token kernel without work costs 4 to 10 us.
+// Sequences with at most `few` new rows are the token kernel's, which reads their pages nearly
+// as fast as memory gives them (64 sequences over 4,000 positions, 4 query heads per kv head:
+// 1 to 4 f16 rows 96 us, 1 to 2 f32 rows over f32 caches 181 us); longer ones the chunk
+// kernel's (1 to 8 f16 rows 147 us, 1 to 5 rows 167 us; 1 to 4 f32 rows over f32 caches 533 us).
+// Both run where short sequences are likely (the longest is far longer than the mean, or the
+// others are short on average; the host does not know) and are more than the chunk kernel
+// would have in one turn of its CTAs, half of that with an f32 cache: 60 tokens over 4,000
+// positions with 4 chunks of 512 rows over 2,000 take 154 us (f16), 202 us (f32 over f16) and
+// 380 us (f32) with both, 202, 321 and 724 us with the chunk kernel alone. 31 tokens over 2,000
+// with a chunk of 256 rows would take 63, 67 and 93 us with both; alone 48, 66 and 148 us: that
+// batch gets both for f32 caches only. A token kernel without work costs 4 to 10 us.
 template <typename T, typename C, int D>
 qora_status launch_attn(paged::AttnArgs a, void* work, cudaStream_t s) {
   a.few = paged::TokenCfg<T, C, D>::kRows / a.group;

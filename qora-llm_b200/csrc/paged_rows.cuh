@@ -18,7 +18,9 @@
 //
 // Measured: norm and rotation of 8,191 bf16 rows of 16 + 4 heads of 128, 88 MB, in 20.5 us =
 // 4.3 TB/s; a warp per head row took 36.9 us, a deeper prefetch and other numbers of blocks
-// per SM were slower. The append of 5 bf16 prompts, 94 MB, 22.7 us. One row: 2.3 us.
+// per SM were slower. The append of 5 bf16 prompts, 94 MB, 22.7 us. A plain copy that moves as
+// many bytes takes 20.4 and 22.6 us (buffers beyond L2, one call after the other): it is the
+// size that keeps these from the bandwidth of long copies. One row: 2.6 us in a graph.
 #pragma once
 
 #include <cuda_bf16.h>

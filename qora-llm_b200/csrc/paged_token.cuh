@@ -33,10 +33,13 @@
 // taken out and added to the rows that do see them, and with NaN scores of f32 rows (an
 // infinite key's product with halves of unlike sign) computed in f32.
 //
-// Measured (graph replays, pages of 16): 128 tokens over up to 4,100 binary16 positions, 1.1
-// GB, 174 us = 6.3 TB/s; 32 tokens over f32 caches, 253 MB, 54 us = 4.7 TB/s; one token over
-// 32,768 binary16 positions, 67 MB, 16 us = 4.1 TB/s, of which some 4 us are the launch, the
-// schedule and the join.
+// Measured, the call replayed in a graph (in brackets: consecutive calls on changing inputs):
+// 128 tokens over 200 to 8,000 binary16 positions, 4,193 on average, 1.1 GB, 175 us = 6.3 TB/s
+// (190 us); 32 tokens over f32 caches, 253 MB, 55 us = 4.6 TB/s (58 us); one token over 32,768
+// binary16 positions, 67 MB, 16 us = 4.1 TB/s (21 us), of which some 4 us are the launch, the
+// schedule and the join. What holds the f32 caches back is the warps' own instructions: the two
+// warps of a scheduler issue in 46 % of its cycles and wait for memory in 7 % of theirs (DRAM 58
+// %, tensor pipe 32 % busy).
 #pragma once
 
 #include "paged_attention.cuh"
@@ -121,7 +124,7 @@ struct TokenCfg {
   // Pieces are permuted within their 128 bytes so that the reads below touch every bank once:
   // ldmatrix reads one piece of 8 rows; a quarter-warp reads 4 pieces of 2 rows of an f32 K
   // and 2 pieces of rows 0, 2, 4, 6 of V. (Rows padded by 16 bytes instead: 225 us where
-  // this takes 196 us, 128 tokens over 4,100 positions each; the copies write whole lines.)
+  // this took 185 us, 128 ragged tokens; the copies write whole lines.)
   QORA_DEV static int k_at(int row, int ch) { return row * kRowBytes + ((kWide ? ch ^ ((row & 1) << 2) : ch ^ (row & 7)) << 4); }
   QORA_DEV static int v_at(int row, int ch) { return row * kRowBytes + ((kWide ? ch ^ (row & 6) : ch ^ (row & 7)) << 4); }
   static constexpr int kSide = kPos * kRowBytes;  // bytes of a step's K (or V)
