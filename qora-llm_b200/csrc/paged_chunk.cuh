@@ -32,7 +32,8 @@
 // thread's products execute in order.
 //
 // f32 operands are split into binary16 upper and lower halves (22 bits) after scaling by a
-// power of two: q by row, K and V by tile (largest value in [2^13, 2^14)). The weights are
+// power of two: q by row, K and V by tile (largest value in [2^13, 2^14); a value less than
+// 2^-15 of that has fewer bits, its error stays within 2^-38 of the largest). The weights are
 // split too. Upper x upper, lower x upper and upper x lower are multiplied: two products
 // instead of one for an f16 cache, three for an f32 cache. The scale of K goes into the
 // scores' scale. 16-bit rows' weights are rounded to the rows' type, which adds about as much

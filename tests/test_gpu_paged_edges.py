@@ -557,3 +557,18 @@ def test_a_captured_batch_of_tokens_and_chunks_grows(pkg, torch, t, kv):
         b.seqs, b.new, b.total = len(live), [new[s] for s in live], [total[s] for s in live]
         b.start, b.table = np.append(b.start[live], b.start[-1]), b.table[live]
         check_on_gpu(torch, b, got, host(lse), q, pool, t, kv, window)
+
+
+@pytest.mark.parametrize("n", [1, 90])
+def test_small_elements_beside_large_ones_in_f32_pages(pkg, torch, n):
+    """window 1: a row is its own position's value. Elements down to 2^-30 of their neighbours keep 22
+    bits or come within 2^-38 of the largest |v| of the 64 positions (single tokens: 22 bits)."""
+    rng = np.random.default_rng(3)
+    b, q, pages, _ = make(torch, rng, "f32", "f32", [n], [300], 16, "slot", 2, 1, 64, extra=0)
+    pages[1] = ref.round_to(np.nan_to_num(pages[1], nan=0.0, posinf=0.0) * 2.0 ** -rng.integers(0, 30, pages[1].shape), "f32")
+    pages[1][..., 0] = 1.0  # rows of like size
+    got, gl, st = attend(pkg, torch, b, q, Pool(torch, "f32", b, 1, 64, "slot", pages), "f32", window=1)
+    v = np.stack([pages[1][b.place(0, p)][0] for p in range(300 - n, 300)])[:, None]
+    floor = 0.0 if n == 1 else 2.0**-38 * np.abs(pages[1]).max()
+    # the weight's halves, the value's halves, the product's sum and the quotient
+    assert st == 0 and np.all(np.abs(got - v) <= (2.0**-21 + 2.0**-22 + 2.0**-22) * np.abs(v) + floor)
