@@ -352,11 +352,11 @@ qora_status qora_q4_lm_head(const float* d_x, const uint8_t* d_packed,
  * together, 16 of bf16); f32 values, and their weights, as two halves of 22 bits together. A
  * weight in binary16 is off by up to 2^-31 of its row's largest (times the largest |v| so far,
  * with f32 pages) where that is more, and a value in halves by up to 2^-38 of the largest of its
- * row (q) or of its head in 64 positions (f32 pages, chunks). The tensor cores cut their f32 sums short, by at most
- * 2^-23 of the magnitudes per position: over all positions for 16-bit rows, over 512 (f32
- * pages: 256) for f32 rows, whose partial sums are added with rounding. Before the division by
- * the sum of the weights these are up to 2^15 times their final size: |v| from 2^90 on may
- * overflow.
+ * row (q) or of its head in 64 positions (f32 pages, chunks). The tensor cores cut their f32
+ * sums short, by at most 2^-23 of the magnitudes per position: over all positions for 16-bit
+ * rows, over 512 (f32 pages: 256) for f32 rows, whose partial sums are added with rounding.
+ * Before the division by the sum of the weights these are up to 2^15 times their final size:
+ * |v| from 2^90 on may overflow.
  *
  * What the host cannot see is checked on the device: a sequence whose rows lie outside
  * [0, rows) or whose length does not fit its table row, a position behind the rotation
